@@ -11,6 +11,9 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = ["api.hip", "gemm.hip", "attention.hip", "elementwise.hip", "engine.hip"]
+# packed fp32 arithmetic (v_pk_add / mul / fma_f32) stays off: hipcc makes it by itself from ordinary float code, and some of its
+# forms have given wrong results on this hardware now and then, without an error
+FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 HEADERS = ["common.h", "gemm_glds_index.h", "gemm_8phase.h", os.path.join("..", "..", "include", "jukebox_hip.h")]
 LIB = os.path.join(HERE, "libjukebox_hip.so")
 LIB_SEGMENTS = os.path.join(HERE, "libjukebox_hip_segments.so")       # measurement build: -DJB_PIPE_SEGMENTS (common.h)
@@ -40,7 +43,7 @@ def build(force=False, verbose=False, segments=False):
     for src in SOURCES:
         obj = os.path.join(HERE, src.replace(".hip", ".seg.o" if segments else ".o"))
         cmd = [_hipcc(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Wall",
-               "-Wno-unused-function"] + (["-DJB_PIPE_SEGMENTS"] if segments else []) + ["-c", os.path.join(HERE, src), "-o", obj]
+               "-Wno-unused-function"] + FLAGS + (["-DJB_PIPE_SEGMENTS"] if segments else []) + ["-c", os.path.join(HERE, src), "-o", obj]
         if verbose:
             print(" ".join(cmd))
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
