@@ -20,7 +20,9 @@ extern "C" {
 typedef enum { JB_F32 = 0, JB_F16 = 1,
                /* jb_pack_weight's dst_dtype only: an fp32 matrix as TWO f16 images, hi = half(w) and lo = half((w - hi) * 2^11),
                 * each in f16 fragment order, hi first -- the weight operand of jb_gemm_args.w_split */
-               JB_F16_SPLIT = 2 } jb_dtype;
+               JB_F16_SPLIT = 2,
+               /* the paged cache's operators and jb_sample_filtered only */
+               JB_BF16 = 3 } jb_dtype;
 typedef enum { JB_OK = 0, JB_ERR_ARG = -1, JB_ERR_UNSUPPORTED = -2, JB_ERR_HIP = -3 } jb_status;
 typedef enum { JB_ACT_NONE = 0, JB_ACT_RELU = 1, JB_ACT_QUICK_GELU = 2 } jb_act;
 
@@ -292,6 +294,39 @@ int jb_vq_gather(const int64_t* codes, const float* codebook, float* out, int64_
  * (BottleneckBlock.quantise, bottleneck.py:112-119). */
 int jb_vq_argmin(const float* x, const float* xk, const float* codebook, int64_t* codes, int64_t rows,
                  int emb_width, int bins, void* stream);
+
+/* ---- keys and values in pages -------------------------------------------------------------------------------------------
+ * A layer's cache as n_pages pages of page_size rows, shared by any number of sequences: a sequence is a row of `table`
+ * (max_pages page numbers in order of position, -1 behind the last) and an entry of `lens` (tokens it holds); `ref` counts, for
+ * every page, the table rows that name it (0: the page is free).  All of them are device arrays of int32, so that a step of
+ * these calls can be captured into a graph and replayed while sequences grow, fork and end. */
+
+/* Attention of every sequence's newest tokens -- cu_q[i+1] - cu_q[i] of them, one or a whole chunk, whose rows the cache already
+ * holds (the last is position lens[i] - 1) -- over its pages.  Replaces what jb_attn_decode / jb_attn_prefill do on a cache of one
+ * fixed length per sample (FactoredAttention.forward(sample=True), jukebox/transformer/factored_attention.py:82-193,289-301).
+ * Rows cu_q[i] .. cu_q[i+1]-1 of q [n_tokens][n_head][d_head] are sequence i's; rows outside every sequence are neither read
+ * nor written.  n_head / n_kv_head consecutive query heads share a key / value head.  A query without a visible key (block 0
+ * of the prev pattern, a length below the number of queries) gives zeros; a masked key or value may hold anything, NaN too;
+ * positions whose table entry is no page number are masked.  Patterns 0-3; `window` (dense only, 0 = off): the query at p sees
+ * positions p - window + 1 .. p.  Strides in elements, channels contiguous; k and v share them.  Softmax in fp32; 16-bit
+ * outputs are rounded once. */
+typedef struct jb_attn_paged_args {
+    int dtype, attn_func;                              /* JB_F32, JB_F16, JB_BF16; of q, k, v and out */
+    const void* q; int64_t q_row_stride, q_head_stride;
+    void* out; int64_t out_row_stride, out_head_stride;
+    const void *k, *v; int64_t page_stride, row_stride, head_stride;
+    int n_pages, page_size;
+    const int* table; int64_t table_stride; int max_pages;
+    const int* lens; const int* cu_q;                  /* [n_seq], [n_seq + 1] */
+    int n_tokens, n_seq, n_head, n_kv_head, d_head;    /* n_tokens: rows of q and out */
+    int max_q, max_len;                                /* the most queries / tokens of a sequence, for the shape of the launch only */
+    int block_ctx, window;
+    float scale;
+    void* workspace; int64_t workspace_bytes;          /* jb_attn_paged_workspace() bytes, 16-byte aligned; holds nothing between calls */
+} jb_attn_paged_args;
+int jb_attn_paged(const jb_attn_paged_args* args /* host */, void* stream);
+/* Bytes of workspace that the call needs (0: none), < 0: a jb_status. */
+int64_t jb_attn_paged_workspace(const jb_attn_paged_args* args /* host */);
 
 /* ---- decode engine: one prior's transformer bound to static buffers ------------------------------ */
 typedef struct jb_layer {

@@ -7,7 +7,7 @@ resolved, `lib()` raises.  Build it with `python -m jukebox_amd.csrc.build` or
 import ctypes as C
 import os
 
-F32, F16, F16_SPLIT = 0, 1, 2
+F32, F16, F16_SPLIT, BF16 = 0, 1, 2, 3
 ACT_NONE, ACT_RELU, ACT_QUICK_GELU = 0, 1, 2
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -47,6 +47,16 @@ class GemvArgs(C.Structure):
 class SampleParams(C.Structure):
     _fields_ = [("temp", f32), ("top_k", i32), ("top_p", f32), ("sample_base", i32), ("seed", C.c_uint64),
                 ("pos_base", i32), ("stream_id", i32)]
+
+
+class AttnPagedArgs(C.Structure):
+    _fields_ = [("dtype", i32), ("attn_func", i32), ("q", vp), ("q_row_stride", i64), ("q_head_stride", i64),
+                ("out", vp), ("out_row_stride", i64), ("out_head_stride", i64),
+                ("k", vp), ("v", vp), ("page_stride", i64), ("row_stride", i64), ("head_stride", i64),
+                ("n_pages", i32), ("page_size", i32), ("table", vp), ("table_stride", i64), ("max_pages", i32),
+                ("lens", vp), ("cu_q", vp), ("n_tokens", i32), ("n_seq", i32), ("n_head", i32), ("n_kv_head", i32),
+                ("d_head", i32), ("max_q", i32), ("max_len", i32), ("block_ctx", i32), ("window", i32), ("scale", f32),
+                ("workspace", vp), ("workspace_bytes", i64)]
 
 
 class Layer(C.Structure):
@@ -107,6 +117,8 @@ _SIGS = {
     "jb_tune_attn_prefill_v2": (None, [i32]),
     "jb_attn_prefill": (i32, [i32, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp]),
     "jb_attn_probs": (i32, [i32, i32, vp, vp, i32, vp, i64, i32, i32, i32, i32, i32, i32, i32, i32, i32, vp]),
+    "jb_attn_paged": (i32, [C.POINTER(AttnPagedArgs), vp]),
+    "jb_attn_paged_workspace": (i64, [C.POINTER(AttnPagedArgs)]),
     "jb_embed": (i32, [i32, vp, vp, i64, vp, vp, vp, i64, vp, i64, i64, i32, i32, i32, vp, i32, vp]),
     "jb_final_add": (i32, [i32, vp, vp, i64, vp, i64, i64, i32, i32, i32, vp, i32, vp]),
     "jb_sample_logits": (i32, [vp, i32, i32, vp, vp, i64, vp, vp, i64, vp]),

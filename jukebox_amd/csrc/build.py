@@ -10,11 +10,11 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = ["api.hip", "gemm.hip", "attention.hip", "elementwise.hip", "engine.hip"]
+SOURCES = ["api.hip", "gemm.hip", "attention.hip", "elementwise.hip", "engine.hip", "paged_attention.hip"]
 # packed fp32 arithmetic (v_pk_add / mul / fma_f32) stays off: hipcc makes it by itself from ordinary float code, and some of its
 # forms have given wrong results on this hardware now and then, without an error
 FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-HEADERS = ["common.h", "gemm_glds_index.h", "gemm_8phase.h", os.path.join("..", "..", "include", "jukebox_hip.h")]
+HEADERS = ["common.h", "paged.h", "gemm_glds_index.h", "gemm_8phase.h", os.path.join("..", "..", "include", "jukebox_hip.h")]
 LIB = os.path.join(HERE, "libjukebox_hip.so")
 LIB_SEGMENTS = os.path.join(HERE, "libjukebox_hip_segments.so")       # measurement build: -DJB_PIPE_SEGMENTS (common.h)
 

@@ -1,0 +1,535 @@
+// Attention of the newest tokens of many sequences over key / value rows that lie in pages.
+//
+//   out[t][h] = sum_k softmax_k(scale q[t][h] . K[k][h / G]) V[k][h / G],   k over the positions that t's position sees
+//
+// A sequence is a row of `table` (its page numbers in order of position) and its length; its queries are its last cu_q[i+1] -
+// cu_q[i] positions.  G = n_head / n_kv_head query heads share a key / value head, so a tile of 16 ROWS -- a row is a (token, head
+// of the group) pair, heads fastest -- meets one K / V stream, for one new token as for thousands.
+#include "paged.h"
+
+namespace {
+
+template <typename T> struct El;
+template <> struct El<f16> {
+    typedef f16x8 vec;
+    static constexpr int E = 8;
+    static constexpr unsigned EXP2 = 0x7c007c00u;
+    static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct El<bf16> {
+    typedef bf16x8 vec;
+    static constexpr int E = 8;
+    static constexpr unsigned EXP2 = 0x7f807f80u;
+    static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct El<float> {
+    typedef f32x4 vec;
+    static constexpr int E = 4;
+    static constexpr unsigned EXP2 = 0x7f800000u;
+    static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return jb_mfma(a, b, c); }
+};
+
+struct Args {
+    const void* q; int64_t q_row, q_head;
+    void* out; int64_t o_row, o_head;
+    const void *k, *v; int64_t page_stride, row_stride, head_stride;
+    const int* table; int64_t table_stride; int max_pages;
+    const int *lens, *cu;
+    float* part; float* ml;                      // splits' states: [token][head][split][D], [token][head][split][2]
+    JbDiv page, group;
+    unsigned n_pages;
+    int page_shift;                              // ceil(log2 page_size): a row of the cache is (page << page_shift) | row in page
+    int n_tokens, n_seq, n_head, n_kv, G, D;
+    int func, bc, window;
+    int tiles, splits; unsigned chunk;                    // grid: row tiles per (sequence, kv head), key splits, keys of a split's turn
+    float c;                                     // scale * log2(e)
+};
+
+constexpr unsigned BAD = 0xffffffffu;            // a key on a page number that does not exist: nobody sees it
+constexpr int KB = 32;                           // keys of a wave's turn
+
+struct Seq { int t0, nq, pos0; const int* table; };      // first query row, queries, position of the first, page numbers
+__device__ __forceinline__ Seq seq_of(const Args& a, int i) {
+    Seq s;
+    s.t0 = min(max(a.cu[i], 0), a.n_tokens);
+    s.nq = max(min(a.cu[i + 1], a.n_tokens) - s.t0, 0);
+    const int64_t cap = (int64_t)a.max_pages * a.page.d;
+    const int len = (int)min((int64_t)max(a.lens[i], 0), min(cap, (int64_t)0x7fff0000));
+    s.pos0 = len - s.nq;
+    s.table = a.table + (int64_t)i * a.table_stride;
+    return s;
+}
+__device__ __forceinline__ int tiles_of(const Args& a, int nq) {
+    if (a.func != JB_ATTN_TRANSPOSE_BLOCK) return (int)(((int64_t)nq * a.G + 15) / 16);
+    const int cls = min(a.bc, nq);
+    return cls == 0 ? 0 : cls * (int)(((int64_t)((nq + a.bc - 1) / a.bc) * a.G + 15) / 16);
+}
+// Row r of a tile is token j0 + i * js of the chunk, i = (row0 + r) / G, head (row0 + r) % G; the keys that any of its rows
+// may see sit at positions kb + x * ks, x < n.
+struct Tile { int j0, js, row0, rows, kb, ks, n; };      // rows: rows of this tile's class in all
+__device__ __forceinline__ Tile tile_of(const Args& a, const Seq& s, int tile) {
+    Tile t;
+    if (a.func == JB_ATTN_TRANSPOSE_BLOCK) {             // one residue class of positions modulo bc
+        const int per = (int)(((int64_t)((s.nq + a.bc - 1) / a.bc) * a.G + 15) / 16);
+        t.j0 = tile / per; t.js = a.bc; t.row0 = (tile % per) * 16;
+        t.rows = (s.nq - t.j0 + a.bc - 1) / a.bc * a.G;
+    } else {
+        t.j0 = 0; t.js = 1; t.row0 = tile * 16; t.rows = s.nq * a.G;
+    }
+    t.kb = 0; t.ks = 1; t.n = 0;
+    if (t.row0 >= t.rows) return t;
+    const int pf = max(s.pos0 + t.j0 + (int)jb_div(t.row0, a.group) * t.js, 0);
+    const int pl = s.pos0 + t.j0 + (int)jb_div(min(t.row0 + 15, t.rows - 1), a.group) * t.js;
+    if (pl < 0) return t;                                // a length shorter than the chunk: no such positions
+    switch (a.func) {
+        case JB_ATTN_BLOCK: t.kb = pf - pf % a.bc; t.n = pl + 1 - t.kb; break;
+        case JB_ATTN_PREV_BLOCK: t.kb = max(pf / a.bc - 1, 0) * a.bc; t.n = max(pl / a.bc * a.bc - t.kb, 0); break;
+        case JB_ATTN_TRANSPOSE_BLOCK: t.ks = a.bc; t.kb = pl % a.bc; t.n = pl / a.bc + 1; break;
+        default: t.kb = a.window ? max(pf - a.window + 1, 0) : 0; t.n = pl + 1 - t.kb;
+    }
+    return t;
+}
+// The positions [lo, hi) that the query at position p sees (of those its tile walks).
+__device__ __forceinline__ void sees(const Args& a, int p, int& lo, int& hi) {
+    lo = 0; hi = p + 1;
+    if (p < 0) { hi = 0; return; }
+    if (a.func == JB_ATTN_BLOCK) lo = p - p % a.bc;
+    else if (a.func == JB_ATTN_PREV_BLOCK) { const int b = p / a.bc; hi = b * a.bc; lo = hi - (b > 0 ? a.bc : 0); }
+    else if (a.func == JB_ATTN_DENSE && a.window) lo = max(p - a.window + 1, 0);
+}
+__device__ __forceinline__ int active_splits(const Args& a, int n) {
+    return a.splits == 1 ? 1 : min(a.splits, max((int)(((unsigned)n + a.chunk - 1u) / a.chunk), 1));
+}
+
+// (page << page_shift) | row in page of a position; BAD where the table names no page.
+__device__ __forceinline__ unsigned cache_row(const Args& a, const Seq& s, int pos) {
+    const unsigned p = jb_div((unsigned)pos, a.page);
+    const unsigned pg = (unsigned)s.table[p];
+    return pg < a.n_pages ? (pg << a.page_shift) | ((unsigned)pos - p * a.page.d) : BAD;
+}
+__device__ __forceinline__ int64_t cache_offset(const Args& a, unsigned row) {
+    row = row == BAD ? 0u : row;
+    return (int64_t)(row >> a.page_shift) * a.page_stride + (int64_t)(row & ((1u << a.page_shift) - 1u)) * a.row_stride;
+}
+template <typename T> __device__ __forceinline__ u32x4 load16(const T* p) { return *reinterpret_cast<const u32x4_any*>(p); }
+
+// The A operands of O^T += V^T P^T from the rows themselves: w[i] holds E consecutive channels of key i of the lane's group, the
+// operand of tile j wants channel j of all of them.  A lane owns both, so the transposition is a byte permutation per two elements.
+__device__ __forceinline__ f16x8 gather(const u32x4 (&w)[8], int j, f16) {
+    u32x4 r;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) r[h] = __builtin_amdgcn_perm(w[2 * h + 1][j >> 1], w[2 * h][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+    return __builtin_bit_cast(f16x8, r);
+}
+__device__ __forceinline__ bf16x8 gather(const u32x4 (&w)[8], int j, bf16) { return __builtin_bit_cast(bf16x8, gather(w, j, f16())); }
+
+template <typename T> __device__ __forceinline__ void store8(T* o, const float* v);
+template <> __device__ __forceinline__ void store8(float* o, const float* v) {
+    *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+    *reinterpret_cast<u32x4_any*>(o + 4) = __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]});
+}
+template <typename T> __device__ __forceinline__ void store8(T* o, const float* v) {
+    typename El<T>::vec x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (T)v[e];
+    *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, x);
+}
+
+// One workgroup of four waves per (sequence, kv head, tile of 16 rows, split of the keys); a wave takes every fourth 32-key turn
+// of its split with a running maximum and sum of its own, and the four states join through LDS.
+//
+//   S^T = K Q^T     A = 16 keys x 32 channels straight from the cache rows, B = the rows' queries (in registers throughout): a
+//                   lane holds, for query row l & 15, the scores of keys (l >> 4) * 4 + r of both 16-key halves -- the softmax
+//                   statistics take two cross-lane steps, and the rescaling of the output none.
+//   O^T += V^T P^T  the order of a product's inner index is free: slot (g, i) is key (i / 4) * 16 + g * 4 + i % 4, so the B
+//                   operand is the lane's own probabilities, and the A operand the lane's own eight value pieces (gather above).
+// K and V therefore go from memory to the matrix cores through registers alone: no LDS, no barrier inside the loop.
+// In 16 bits the probabilities enter as a high and a low part (two products): the output is as near the 64-bit value as its own
+// rounding allows; the products hide behind the memory anyway (one new token: 1 row of 16 used).
+// NC: chunks of 16 E channels that cover d_head.
+template <typename T, int NC>
+__global__ __launch_bounds__(256) void attn_paged_rows_kernel(const Args a) {
+    typedef typename El<T>::vec vec;
+    constexpr int E = El<T>::E, CH = 16 * E, KT = 4 * E, NK = NC * CH / KT;
+    constexpr bool WIDE = NC * E > 8;
+    constexpr int LDO = CH + 4;                  // floats between two rows of the exchange: rows 4 banks apart
+    __shared__ float s_o[4][16][LDO];
+    __shared__ float s_ml[4][16][2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    int64_t b = blockIdx.x;
+    const int tile0 = (int)(b % a.tiles); b /= a.tiles;
+    const int split = (int)(b % a.splits); b /= a.splits;
+    const int kvh = (int)(b % a.n_kv), si = (int)(b / a.n_kv);
+    const Seq s = seq_of(a, si);
+    const int n_tiles = tiles_of(a, s.nq);
+    const T* kbase = (const T*)a.k + (int64_t)kvh * a.head_stride;
+    const T* vbase = (const T*)a.v + (int64_t)kvh * a.head_stride;
+    const int D = a.D, nk = (D + KT - 1) / KT;
+
+    for (int tile = tile0; tile < n_tiles; tile += a.tiles) {
+        const Tile t = tile_of(a, s, tile);
+        if (t.row0 >= t.rows) continue;
+        const int n_act = active_splits(a, t.n);
+        if (split >= n_act) continue;
+        const int R = t.row0 + c, my = min(R, t.rows - 1);
+        const int qi = (int)jb_div(my, a.group), j = t.j0 + qi * t.js, head = kvh * a.G + (my - qi * a.G);
+        const bool row_ok = R < t.rows;
+        int lo, hi;
+        sees(a, s.pos0 + j, lo, hi);
+        if (!row_ok) hi = lo;
+        // positions that every row of the tile sees: the first row ends first, the last begins last
+        int all_lo, all_hi, dummy;
+        sees(a, s.pos0 + t.j0 + (int)jb_div(t.row0, a.group) * t.js, dummy, all_hi);
+        sees(a, s.pos0 + t.j0 + (int)jb_div(min(t.row0 + 15, t.rows - 1), a.group) * t.js, all_lo, dummy);
+
+        const T* qrow = (const T*)a.q + (int64_t)(s.t0 + j) * a.q_row + (int64_t)head * a.q_head;
+        vec qf[NK];
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+            // a fragment that passes the end of the head is read from D - E on, as the keys' is; what an earlier one covers is zeroed
+            const int e0 = ks * KT + g * E, at = min(e0, D - E);
+            qf[ks] = __builtin_bit_cast(vec, load16(qrow + at));
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (at + e < e0 || !row_ok) qf[ks][e] = (T)0.f;
+        }
+        f32x4 acc[NC][E];
+#pragma unroll
+        for (int ch = 0; ch < NC; ++ch)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[ch][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;            // of the lane's row, the same in its four lanes
+
+        for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
+            const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n);
+            for (int xb = (int)x0 + wave * KB; xb < x1; xb += 4 * KB) {
+                const int xl = min(xb + (lane & 31), x1 - 1);
+                const unsigned row = cache_row(a, s, t.kb + xl * t.ks);
+                unsigned vrow[8];
+                const T* kp[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) kp[h] = kbase + cache_offset(a, __shfl(row, h * 16 + c));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) vrow[i] = __shfl(row, (i >> 2) * 16 + g * 4 + (i & 3));
+                // narrow heads ask for all keys and values of the turn together; wide ones, which the registers do not hold at
+                // once, for a half of the keys, then the other, then the values 16 E channels at a time
+                u32x4 kf[WIDE ? 1 : 2][NK], vf[WIDE ? 1 : NC][8];
+                f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+                auto load_k = [&](int h) {
+#pragma unroll
+                    for (int ks = 0; ks < NK; ++ks)
+                        if (ks < nk) kf[WIDE ? 0 : h][ks] = load16(kp[h] + min(ks * KT + g * E, D - E));
+                };
+                auto load_v = [&](int ch) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) vf[WIDE ? 0 : ch][i] = load16(vbase + cache_offset(a, vrow[i]) + min(ch * CH + c * E, D - E));
+                };
+                auto score = [&](int h) {
+#pragma unroll
+                    for (int ks = 0; ks < NK; ++ks)
+                        if (ks < nk) sc[h] = El<T>::mfma(__builtin_bit_cast(vec, kf[WIDE ? 0 : h][ks]), qf[ks], sc[h]);
+                };
+                load_k(0);
+                if constexpr (WIDE) score(0);
+                load_k(1);
+                if constexpr (!WIDE) {
+#pragma unroll
+                    for (int ch = 0; ch < NC; ++ch) load_v(ch);
+                    score(0);
+                }
+                score(1);
+                // scores of keys h * 16 + g * 4 + r, i.e. of slot i = h * 4 + r
+                const int p0 = t.kb + xb * t.ks, p1 = t.kb + (xb + KB - 1) * t.ks;
+                const bool masked = xb + KB > x1 || p0 < all_lo || p1 >= all_hi || t.rows - t.row0 < 16 || __any(row == BAD);
+                unsigned see = 0xffu;
+                if (masked) {
+                    see = 0u;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int x = xb + (i >> 2) * 16 + g * 4 + (i & 3), p = t.kb + x * t.ks;
+                        if (x < x1 && p >= lo && p < hi && vrow[i] != BAD) see |= 1u << i;
+                    }
+                }
+                float p[8], mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    p[i] = (see >> i) & 1u ? sc[i >> 2][i & 3] * a.c : -INFINITY;
+                    mx = fmaxf(mx, p[i]);
+                }
+                mx = jb_rows_reduce(mx, [](float u, float v) { return fmaxf(u, v); });
+                const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.f : m_new;
+                const float alpha = __builtin_amdgcn_exp2f(m - base);
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { p[i] = __builtin_amdgcn_exp2f(p[i] - base); sum += p[i]; }
+                sum = jb_rows_reduce(sum, [](float u, float v) { return u + v; });
+                l = l * alpha + sum;
+                m = m_new;
+                if (__any(alpha != 1.0f)) {
+#pragma unroll
+                    for (int ch = 0; ch < NC; ++ch)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) acc[ch][e] *= alpha;
+                }
+                // A value that is no number may sit in a row that some queries do not see, and 0 * NaN would reach them.  Where a
+                // turn is masked at all its values are looked at: such elements leave the operands, and enter below one key at a
+                // time, for the queries that see it.
+                unsigned odd = 0u;
+                vec ph, pl;
+                if constexpr (E == 8) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { ph[i] = (T)p[i]; pl[i] = (T)(p[i] - (float)ph[i]); }
+                }
+#pragma unroll
+                for (int ch = 0; ch < NC; ++ch) {
+                    if (ch * CH >= D) break;
+                    if constexpr (WIDE) load_v(ch);
+                    u32x4 (&w)[8] = vf[WIDE ? 0 : ch];
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+                                const unsigned x = w[i][h] & El<T>::EXP2;
+                                if constexpr (E == 4) {
+                                    if (x == El<T>::EXP2) { odd |= 1u << i; w[i][h] = 0u; }
+                                } else {
+                                    const bool b0 = (x & 0xffffu) == (El<T>::EXP2 & 0xffffu), b1 = x >> 16 == El<T>::EXP2 >> 16;
+                                    if (b0 || b1) { odd |= 1u << i; w[i][h] &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0xffffu : 0xffffffffu); }
+                                }
+                            }
+                    }
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        if constexpr (E == 8) {
+                            const vec vt = gather(w, e, T());
+                            acc[ch][e] = El<T>::mfma(vt, ph, acc[ch][e]);
+                            acc[ch][e] = El<T>::mfma(vt, pl, acc[ch][e]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                acc[ch][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, w[i])[e], p[i], acc[ch][e], 0, 0, 0);
+                        }
+                    }
+                }
+                if (__any(odd != 0u)) {
+                    for (int i = 0; i < 8; ++i) {
+                        const unsigned long long who = __ballot(odd >> i & 1u);
+                        float pi = p[0];
+                        unsigned ri = vrow[0];
+#pragma unroll
+                        for (int u = 1; u < 8; ++u) { pi = u == i ? p[u] : pi; ri = u == i ? vrow[u] : ri; }
+                        for (int gg = 0; gg < 4; ++gg) {
+                            if ((who >> (16 * gg) & 0xffffull) == 0) continue;
+                            const float pk = __shfl(pi, gg * 16 + c);
+                            const bool take = __shfl(see, gg * 16 + c) >> i & 1u;
+                            const T* vp = vbase + cache_offset(a, __shfl(ri, gg * 16));
+#pragma unroll
+                            for (int ch = 0; ch < NC; ++ch)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    const vec w = __builtin_bit_cast(vec, load16(vp + min(ch * CH + (g * 4 + r) * E, D - E)));
+#pragma unroll
+                                    for (int e = 0; e < E; ++e) {
+                                        const float x = (float)w[e];
+                                        if (take && !(fabsf(x) < INFINITY)) acc[ch][e][r] += pk * x;
+                                    }
+                                }
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- join the four waves' states -----------------------------------------------------------
+        __syncthreads();                          // the exchange of the previous tile has been read
+        if (g == 0) { s_ml[wave][c][0] = m; s_ml[wave][c][1] = l; }
+        __syncthreads();
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, s_ml[w][c][0]);
+        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) L += s_ml[w][c][1] * __builtin_amdgcn_exp2f(s_ml[w][c][0] - base);
+        const float mine = __builtin_amdgcn_exp2f(m - base);
+        const float inv = n_act > 1 ? 1.f : L != 0.f ? 1.f / L : 0.f;         // nothing seen: zeros
+        // what this thread writes: E channels from ch * CH + (tid % 16) * E of row tid / 16
+        const int wr = threadIdx.x >> 4, wc = threadIdx.x & 15;
+        const int wR = t.row0 + wr, wi = (int)jb_div(min(wR, t.rows - 1), a.group);
+        const int64_t wt = s.t0 + t.j0 + wi * t.js;
+        const int wh = kvh * a.G + (min(wR, t.rows - 1) - wi * a.G);
+        if (n_act > 1 && wave == 0 && g == 0 && row_ok) {
+            float* o = a.ml + (((int64_t)(s.t0 + j) * a.n_head + head) * a.splits + split) * 2;
+            o[0] = M; o[1] = L;
+        }
+#pragma unroll
+        for (int ch = 0; ch < NC; ++ch) {
+            if (ch * CH >= D) break;
+            if (ch) __syncthreads();
+            // a lane holds channels of pieces g * 4 + r: piece m's tile e is channel min(ch * CH + m * E, D - E) + e
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                for (int e = 0; e < E; e += 4) {
+                    *reinterpret_cast<f32x4*>(&s_o[wave][c][(g * 4 + r) * E + e]) =
+                        f32x4{acc[ch][e][r], acc[ch][e + 1][r], acc[ch][e + 2][r], acc[ch][e + 3][r]} * (mine * inv);
+                }
+            }
+            __syncthreads();
+            const int d0 = ch * CH + wc * E, at = min(d0, D - E);
+            if (wR < t.rows && d0 < D) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = (s_o[0][wr][wc * E + e] + s_o[1][wr][wc * E + e]) + (s_o[2][wr][wc * E + e] + s_o[3][wr][wc * E + e]);
+                if (n_act > 1) {
+                    float* o = a.part + (((wt * a.n_head + wh) * a.splits + split) * (int64_t)D + at);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = v[e];
+                } else {
+                    T* o = (T*)a.out + wt * a.o_row + (int64_t)wh * a.o_head + at;
+                    if constexpr (E == 8) store8<T>(o, v);
+                    else *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+                }
+            }
+        }
+    }
+}
+
+// Joins the splits' states of rows that were split: one workgroup per (sequence, kv head, tile), 16 threads a row.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(const Args a) {
+    int64_t b = blockIdx.x;
+    const int tile0 = (int)(b % a.tiles); b /= a.tiles;
+    const int kvh = (int)(b % a.n_kv), si = (int)(b / a.n_kv);
+    const Seq s = seq_of(a, si);
+    const int n_tiles = tiles_of(a, s.nq), wr = threadIdx.x >> 4, wc = threadIdx.x & 15;
+    for (int tile = tile0; tile < n_tiles; tile += a.tiles) {
+        const Tile t = tile_of(a, s, tile);
+        const int R = t.row0 + wr, n_act = active_splits(a, t.n);
+        if (R >= t.rows || n_act < 2) continue;
+        const int i = (int)jb_div(R, a.group);
+        const int64_t tok = s.t0 + t.j0 + i * t.js;
+        const int h = kvh * a.G + (R - i * a.G);
+        const float* ml = a.ml + (tok * a.n_head + h) * a.splits * 2;
+        const float* part = a.part + (tok * a.n_head + h) * a.splits * (int64_t)a.D;
+        float M = -INFINITY, L = 0.f;
+        for (int u = 0; u < n_act; ++u) M = fmaxf(M, ml[2 * u]);
+        const float base = M == -INFINITY ? 0.f : M;
+        for (int u = 0; u < n_act; ++u) L += ml[2 * u + 1] * __builtin_amdgcn_exp2f(ml[2 * u] - base);
+        const float inv = L != 0.f ? 1.f / L : 0.f;
+        T* o = (T*)a.out + tok * a.o_row + (int64_t)h * a.o_head;
+        for (int d = wc; d < a.D; d += 16) {
+            float v = 0.f;
+            for (int u = 0; u < n_act; ++u) v += part[(int64_t)u * a.D + d] * __builtin_amdgcn_exp2f(ml[2 * u] - base);
+            o[d] = (T)(v * inv);
+        }
+    }
+}
+
+struct Plan { int64_t tiles, range; int splits; unsigned chunk; };
+Plan plan_of(const jb_attn_paged_args* p) {
+    Plan w;
+    const int64_t G = p->n_head / p->n_kv_head, bc = p->block_ctx;
+    if (p->attn_func == JB_ATTN_TRANSPOSE_BLOCK) w.tiles = (int64_t)(p->max_q < bc ? p->max_q : bc) * (((p->max_q + bc - 1) / bc * G + 15) / 16);
+    else w.tiles = (p->max_q * G + 15) / 16;
+    // keys that a tile walks at most
+    w.range = p->max_len;
+    if (p->attn_func == JB_ATTN_BLOCK || p->attn_func == JB_ATTN_PREV_BLOCK) w.range = bc + 16 / G;
+    else if (p->attn_func == JB_ATTN_TRANSPOSE_BLOCK) w.range = (p->max_len + bc - 1) / bc;
+    else if (p->window) w.range = (int64_t)p->window + 16 / G;
+    if (w.range > p->max_len) w.range = p->max_len;
+    const int64_t wgs = w.tiles * p->n_kv_head * p->n_seq;
+    w.splits = 1; w.chunk = 0x7fffffff;
+    if (wgs < 1024 && w.range > 256) {
+        int64_t chunk = (wgs * w.range / 2048 + 127) / 128 * 128;
+        if (chunk < 256) chunk = 256;
+        if ((w.range + chunk - 1) / chunk > 64) chunk = ((w.range + 63) / 64 + 127) / 128 * 128;
+        w.splits = (int)((w.range + chunk - 1) / chunk);
+        w.chunk = (unsigned)chunk;
+        if (w.splits < 2) { w.splits = 1; w.chunk = 0x7fffffff; }
+    }
+    return w;
+}
+int64_t workspace_of(const jb_attn_paged_args* p, const Plan& w) {
+    return w.splits == 1 ? 0 : (int64_t)p->n_tokens * p->n_head * w.splits * (p->d_head + 2) * 4;
+}
+
+int check_args(const jb_attn_paged_args* a, const char* who) {
+    auto bad = [&](const char* what) { jb_set_error(std::string(who) + ": " + what); return (int)JB_ERR_ARG; };
+    if (!a) return bad("null pointer");
+    if (a->dtype != JB_F32 && a->dtype != JB_F16 && a->dtype != JB_BF16) return bad("bad dtype");
+    if (a->attn_func < JB_ATTN_DENSE || a->attn_func > JB_ATTN_PREV_BLOCK) {
+        jb_set_error(std::string(who) + ": pages hold the keys of dense, block, transpose and prev layers");
+        return JB_ERR_UNSUPPORTED;
+    }
+    if (a->n_tokens < 0 || a->n_seq < 0 || a->n_head <= 0 || a->n_kv_head <= 0 || a->n_head % a->n_kv_head) return bad("bad dims");
+    if (a->d_head < 8 || a->d_head > 512) { jb_set_error(std::string(who) + ": heads of 8 to 512 channels"); return JB_ERR_UNSUPPORTED; }
+    if (a->n_pages <= 0 || a->page_size <= 0 || a->max_pages <= 0) return bad("bad dims of the cache");
+    int sh = 0;
+    while (sh < 31 && (1 << sh) < a->page_size) ++sh;
+    if (((uint64_t)a->n_pages << sh) > 0xffffffffull || (int64_t)a->n_pages * a->page_size > 0x7fffffff) return bad("more than 2^31 cache rows");
+    if (a->page_stride < 0 || a->row_stride < 0 || a->head_stride < 0 || a->q_row_stride < 0 || a->q_head_stride < 0 || a->table_stride < 0) return bad("negative stride");
+    if (a->out_head_stride < a->d_head || a->out_row_stride < a->d_head) return bad("output rows overlap");
+    if (a->attn_func != JB_ATTN_DENSE && a->block_ctx <= 0) return bad("block_ctx required");
+    if (a->window < 0 || (a->window && a->attn_func != JB_ATTN_DENSE)) return bad("a window goes with the dense pattern");
+    if (a->max_q < 0 || a->max_len < 0 || (int64_t)a->max_q * a->n_head > 0x7fffffff || (int64_t)a->n_tokens * a->n_head > 0x7fffffff) return bad("bad dims");
+    return JB_OK;
+}
+
+template <typename T, int NC> void launch_rows(const Args& k, int64_t wgs, hipStream_t s) {
+    attn_paged_rows_kernel<T, NC><<<(unsigned)wgs, 256, 0, s>>>(k);
+}
+
+}  // namespace
+
+extern "C" int64_t jb_attn_paged_workspace(const jb_attn_paged_args* a) {
+    const int rc = check_args(a, __func__);
+    if (rc) return rc;
+    if (a->n_tokens == 0 || a->n_seq == 0 || a->max_q == 0) return 0;
+    return workspace_of(a, plan_of(a));
+}
+
+extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
+    const int rc = check_args(a, __func__);
+    if (rc) return rc;
+    if (a->n_tokens == 0 || a->n_seq == 0 || a->max_q == 0) return JB_OK;
+    JB_REQUIRE(a->q && a->k && a->v && a->out && a->table && a->lens && a->cu_q, "null pointer");
+    const Plan w = plan_of(a);
+    const int64_t need = workspace_of(a, w);
+    JB_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need && (uintptr_t)a->workspace % 16 == 0), "workspace missing, too small or not aligned");
+    const int64_t wgs = w.tiles * a->n_kv_head * a->n_seq;
+    JB_REQUIRE(wgs * w.splits <= 0x7fffffff, "grid too large");
+    Args k = {};
+    k.q = a->q; k.q_row = a->q_row_stride; k.q_head = a->q_head_stride;
+    k.out = a->out; k.o_row = a->out_row_stride; k.o_head = a->out_head_stride;
+    k.k = a->k; k.v = a->v; k.page_stride = a->page_stride; k.row_stride = a->row_stride; k.head_stride = a->head_stride;
+    k.table = a->table; k.table_stride = a->table_stride; k.max_pages = a->max_pages;
+    k.lens = a->lens; k.cu = a->cu_q;
+    k.page = jb_make_div((unsigned)a->page_size);
+    k.group = jb_make_div((unsigned)(a->n_head / a->n_kv_head));
+    k.n_pages = (unsigned)a->n_pages;
+    while ((1 << k.page_shift) < a->page_size) ++k.page_shift;
+    k.n_tokens = a->n_tokens; k.n_seq = a->n_seq; k.n_head = a->n_head; k.n_kv = a->n_kv_head; k.G = a->n_head / a->n_kv_head; k.D = a->d_head;
+    k.func = a->attn_func; k.bc = a->block_ctx > 0 ? a->block_ctx : 1; k.window = a->window;
+    k.tiles = (int)w.tiles; k.splits = w.splits; k.chunk = w.chunk;
+    k.c = a->scale * 1.44269504088896340736f;
+    if (need) {
+        k.part = (float*)a->workspace;
+        k.ml = k.part + (int64_t)a->n_tokens * a->n_head * w.splits * a->d_head;
+    }
+    hipStream_t s = (hipStream_t)stream;
+#define JB_ROWS(T, CH)                                                            \
+    do {                                                                          \
+        if (a->d_head <= 128) launch_rows<T, 128 / CH>(k, wgs * w.splits, s);     \
+        else if (a->d_head <= 256) launch_rows<T, 256 / CH>(k, wgs * w.splits, s);\
+        else launch_rows<T, 512 / CH>(k, wgs * w.splits, s);                      \
+        JB_CHECK_LAUNCH();                                                        \
+        if (w.splits > 1) attn_paged_join_kernel<T><<<(unsigned)wgs, 256, 0, s>>>(k); \
+    } while (0)
+    if (a->dtype == JB_F16) JB_ROWS(f16, 128);
+    else if (a->dtype == JB_BF16) JB_ROWS(bf16, 128);
+    else JB_ROWS(float, 64);
+#undef JB_ROWS
+    JB_CHECK_LAUNCH();
+    return JB_OK;
+}

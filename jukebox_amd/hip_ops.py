@@ -302,6 +302,91 @@ def attn_prefill(func, q, kcache, vcache, n_head, block_ctx, t0):
     return out
 
 
+# ---- keys and values in pages ---------------------------------------------------------------------------------------------
+
+_PAGED_TYPES = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
+
+
+def _paged_type(*ts):
+    """dtype code of the paged cache's operators (single, half and bfloat16) for tensors that must share it."""
+    code = _PAGED_TYPES.get(ts[0].dtype)
+    if code is None or any(t.dtype != ts[0].dtype for t in ts):
+        raise L.JukeboxHipError(f"expected one type of float32, float16, bfloat16; got {', '.join(str(t.dtype) for t in ts)}")
+    return code
+
+
+def _chk_paged(first, *ts):
+    """Every tensor on the first one's GPU."""
+    if not first.is_cuda or any(t is not None and t.device != first.device for t in ts):
+        raise L.JukeboxHipError("expected tensors on one GPU")
+
+
+def _chk_int(name, t, *shape):
+    """A contiguous int32 array; None in `shape`: any length."""
+    if t.dtype != torch.int32 or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)) or not t.is_contiguous():
+        raise L.JukeboxHipError(f"{name}: expected a contiguous int32 array of shape {tuple('*' if n is None else n for n in shape)}")
+
+
+def _chk_table(table):
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] == 0 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise L.JukeboxHipError("table: expected int32 rows of page numbers")
+    # rows of a table of one row may carry any stride
+    stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    if stride < table.shape[1]:
+        raise L.JukeboxHipError("table: rows overlap")
+    return stride
+
+
+def _launch(fn, device, *args):
+    """A call of the library on the current stream of the tensors' own GPU."""
+    if device.index == torch.cuda.current_device():
+        L.check(fn(*args, L.stream()))
+    else:
+        with torch.cuda.device(device):
+            L.check(fn(*args, L.stream()))
+
+
+def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, func=0, block_ctx=0, window=0, scale=None, out=None):
+    """Attention of every sequence's newest tokens over keys and values in pages (jb_attn_paged).
+
+    q (n_tokens, n_head, d_head): rows cu_q[i] .. cu_q[i + 1] - 1 are the last positions of sequence i, whose keys and values
+    the cache holds already.  kpool, vpool (n_pages, page_size, n_kv_head, d_head), any strides that both share, channels
+    contiguous.  table (n_seq, max_pages), lens (n_seq), cu_q (n_seq + 1): int32 on the GPU.  max_q, max_len: the most queries
+    / tokens of a sequence, which shape the launch (default: all rows of q, all of the table's pages).  func, block_ctx: the
+    pattern (dense, block, transpose, prev); window: the query at position p sees p - window + 1 .. p (dense).  scale:
+    1 / sqrt(d_head) by default.  Returns (n_tokens, n_head, d_head); with `out`, rows outside every sequence stay as they are."""
+    code = _paged_type(q, kpool, vpool)
+    _chk_paged(q, kpool, vpool, table, lens, cu_q, out)
+    if q.dim() != 3 or kpool.dim() != 4 or kpool.shape != vpool.shape or kpool.stride() != vpool.stride() or q.shape[2] != kpool.shape[3]:
+        raise L.JukeboxHipError("expected q (n_tokens, n_head, d_head) and kpool, vpool (n_pages, page_size, n_kv_head, d_head) of equal strides")
+    T, H, D = q.shape
+    P, page, KV, _ = kpool.shape
+    table_stride = _chk_table(table)
+    n = table.shape[0]
+    _chk_int("lens", lens, n)
+    _chk_int("cu_q", cu_q, n + 1)
+    if out is None:
+        out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise L.JukeboxHipError("out: expected q's shape and type")
+    if q.stride(2) != 1 or kpool.stride(3) != 1 or out.stride(2) != 1:
+        raise L.JukeboxHipError("expected contiguous channels")
+    ps, rs, hs = kpool.stride()[:3]
+    a = L.AttnPagedArgs(code, func, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0) if T > 1 else H * D,
+                        out.stride(1) if H > 1 else D, kpool.data_ptr(), vpool.data_ptr(), ps, rs, hs, P, page, table.data_ptr(),
+                        table_stride, table.shape[1], lens.data_ptr(), cu_q.data_ptr(), T, n, H, KV, D, T if max_q is None else min(max_q, T),
+                        min(table.shape[1] * page if max_len is None else max_len, 0x7fffffff), block_ctx or 0, window or 0,
+                        1.0 / math.sqrt(D) if scale is None else scale, None, 0)
+    need = L.lib().jb_attn_paged_workspace(C.byref(a))
+    if need < 0:
+        L.check(need)
+    if need:            # the caching allocator keeps it for this stream (or this captured graph) until the launches have run
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    _launch(L.lib().jb_attn_paged, q.device, C.byref(a))
+    return out
+
+
 def vq_gather(codes, codebook):
     """(N, T) int64 -> (N, T, emb) fp32 (BottleneckBlock.decode, channels-last)."""
     _chk_cuda(codes, codebook)
