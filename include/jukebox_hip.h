@@ -285,6 +285,25 @@ int jb_sample_step(const float* logits, int n_batch, int bins, const jb_sample_p
                    const float* x_emb, const float* pos_emb, const float* x_cond, int64_t xc_n_stride, int64_t xc_t_stride,
                    int width, int seq_len, unsigned* ticket, void* stream);
 
+/* One token a row from given uniform numbers: temperature, then top-k, top-p and min-p, then the draw -- what jb_sample_logits does
+ * with a generator of its own, one filter at a time and up to 4096 bins (filter_logits, jukebox/transformer/ops.py:113-142), for any
+ * vocabulary of up to 262144 tokens, every row with settings of its own.  With w_i = exp((x_i - max) / temp) and the row ordered by
+ * falling logit, equal ones by rising index: top-k keeps the first k (k <= 0 or >= bins: off); top-p, of those, each entry before
+ * which the weights sum to at most p of theirs (p <= 0 or >= 1: off); min-p those with w_i >= min_p (<= 0: off; above 1 is 1).
+ * The token is the first index at which the sum of kept weights, by rising index, exceeds u times their total.  temp <= 0: the
+ * largest logit, the lowest index of equal ones.  -inf and NaN are forbidden tokens; a row of nothing else gives -1.  u below 0 (NaN)
+ * counts as 0, from 1 on as the last kept token.  Weights and sums are exact to 2^-45 of the largest weight: the answer is the
+ * definition's in 64 bits, whatever the order of summation; weights below 2^-45 (logits 31.2 temp under the largest) are 0. */
+typedef struct jb_sample_filtered_args {
+    int dtype;                                         /* JB_F32, JB_F16, JB_BF16 */
+    const void* logits; int64_t ld; int rows, bins;    /* [rows] of ld elements, bins of them logits */
+    const float* u;                                    /* [rows], in [0, 1) */
+    const float* temp; const int* top_k; const float *top_p, *min_p;              /* [rows] each, or NULL: */
+    float temp_all; int top_k_all; float top_p_all, min_p_all;                    /* the value of every row */
+    int64_t* tokens;                                   /* [rows] */
+} jb_sample_filtered_args;
+int jb_sample_filtered(const jb_sample_filtered_args* args /* host */, void* stream);
+
 /* Codebook gather (BottleneckBlock.dequantise/decode, jukebox/vqvae/bottleneck.py:121-123,138-147),
  * output channels-last rows [n*T][emb_width] fp32. */
 int jb_vq_gather(const int64_t* codes, const float* codebook, float* out, int64_t n_codes, int emb_width, int bins,
@@ -327,6 +346,49 @@ typedef struct jb_attn_paged_args {
 int jb_attn_paged(const jb_attn_paged_args* args /* host */, void* stream);
 /* Bytes of workspace that the call needs (0: none), < 0: a jb_status. */
 int64_t jb_attn_paged_workspace(const jb_attn_paged_args* args /* host */);
+
+/* New rows into the pages: row t of k and v [n_tokens][n_kv_head][d_head] to cache row slots[t] = page * page_size + row in the
+ * page (jb_pages_extend makes them); rows with a slot outside the cache -- -1 -- are not written.  No slot twice.  Strides in
+ * elements, channels contiguous, k and v alike.  What jb_gemm's qkv_split does for the fixed caches. */
+typedef struct jb_kv_write_args {
+    int dtype;
+    const void *k, *v; int64_t tok_stride, tok_head_stride;
+    void *kpool, *vpool; int64_t page_stride, row_stride, head_stride;
+    int n_pages, page_size;
+    const int64_t* slots;
+    int n_tokens, n_kv_head, d_head;
+} jb_kv_write_args;
+int jb_kv_write(const jb_kv_write_args* args /* host */, void* stream);
+
+/* Control of the pages.  Free pages are given out from the lowest number on: what a call does depends on its arguments alone.
+ * A call that cannot be done changes nothing but *status (device int, never reset by the library): JB_PAGES_NONE_FREE if there
+ * are not enough free pages, JB_PAGES_BAD_ARG if a row lies outside the table or is named twice, if a length is negative or
+ * does not fit the table's row, or if the offsets are not ascending from 0.  `work`: device scratch of the int32s that each call names;
+ * holds nothing between calls. */
+enum { JB_PAGES_NONE_FREE = 1, JB_PAGES_BAD_ARG = 2 };
+typedef struct jb_page_table {
+    int* table; int64_t table_stride; int n_seq, max_pages;
+    int* lens; int* ref; int n_pages, page_size;
+} jb_page_table;
+/* n_pools arrays of n_pages pages -- a layer's keys are one, its values another --, page i at base + i * page_stride bytes */
+typedef struct jb_page_pools {
+    void* const* base /* host array */; int n_pools, n_pages; int64_t page_bytes, page_stride;
+} jb_page_pools;
+/* Room for cu_new[i+1] - cu_new[i] more tokens of every sequence: pages are taken, lens grows, and slots[t] is the cache row of
+ * new token t (-1 behind the last token, and for every token if the call could not be done).  work: 1 + 2 n_seq + n_pages. */
+int jb_pages_extend(const jb_page_table* table /* host */, const int* cu_new, int n_tokens, int64_t* slots, int* work, int* status, void* stream);
+/* The sequences in these rows end: their pages lose a reference each, the rows become -1 and the lengths 0. */
+int jb_pages_free(const jb_page_table* table /* host */, const int* rows, int n_rows, int* status, void* stream);
+/* Sequence dst[i] becomes a fork of src[i]: it shares the full pages (a reference more each) and gets a copy of the last, part-filled
+ * one, in every pool, so that either may grow.  The rows dst must be empty (length 0), and none of them a source.  work: 2 + 4 n_pairs. */
+int jb_pages_fork(const jb_page_table* table /* host */, const jb_page_pools* pools /* host */, const int* src, const int* dst, int n_pairs,
+                  int* work, int* status, void* stream);
+/* The live pages (ref > 0) move to the numbers 0 .. live - 1 in every pool: of those at or above, the lowest goes to the lowest free
+ * number, and so on.  table_out [n_seq][max_pages] and ref_out [n_pages] are the table and the counts afterwards; table and ref stay
+ * as they are (lens is not looked at).  work: 2 + 3 n_pages. */
+int jb_pages_compact(const jb_page_table* table /* host */, const jb_page_pools* pools /* host */, int* table_out, int* ref_out, int* work, void* stream);
+/* Page src[i] of every pool to page dst[i]; pairs outside the pool are skipped.  No target twice, no target that is a source. */
+int jb_pages_copy(const jb_page_pools* pools /* host */, const int* src, const int* dst, int n_pairs, void* stream);
 
 /* ---- decode engine: one prior's transformer bound to static buffers ------------------------------ */
 typedef struct jb_layer {

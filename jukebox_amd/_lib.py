@@ -59,6 +59,26 @@ class AttnPagedArgs(C.Structure):
                 ("workspace", vp), ("workspace_bytes", i64)]
 
 
+class KvWriteArgs(C.Structure):
+    _fields_ = [("dtype", i32), ("k", vp), ("v", vp), ("tok_stride", i64), ("tok_head_stride", i64),
+                ("kpool", vp), ("vpool", vp), ("page_stride", i64), ("row_stride", i64), ("head_stride", i64),
+                ("n_pages", i32), ("page_size", i32), ("slots", vp), ("n_tokens", i32), ("n_kv_head", i32), ("d_head", i32)]
+
+
+class PageTable(C.Structure):
+    _fields_ = [("table", vp), ("table_stride", i64), ("n_seq", i32), ("max_pages", i32), ("lens", vp), ("ref", vp),
+                ("n_pages", i32), ("page_size", i32)]
+
+
+class PagePools(C.Structure):
+    _fields_ = [("base", C.POINTER(vp)), ("n_pools", i32), ("n_pages", i32), ("page_bytes", i64), ("page_stride", i64)]
+
+
+class SampleFilteredArgs(C.Structure):
+    _fields_ = [("dtype", i32), ("logits", vp), ("ld", i64), ("rows", i32), ("bins", i32), ("u", vp), ("temp", vp), ("top_k", vp),
+                ("top_p", vp), ("min_p", vp), ("temp_all", f32), ("top_k_all", i32), ("top_p_all", f32), ("min_p_all", f32), ("tokens", vp)]
+
+
 class Layer(C.Structure):
     _fields_ = [("attn_func", i32), ("w_attn", vp), ("w_proj", vp), ("w_fc", vp), ("w_proj2", vp),
                 ("b_attn", vp), ("b_proj", vp), ("b_fc", vp), ("b_proj2", vp),
@@ -119,6 +139,13 @@ _SIGS = {
     "jb_attn_probs": (i32, [i32, i32, vp, vp, i32, vp, i64, i32, i32, i32, i32, i32, i32, i32, i32, i32, vp]),
     "jb_attn_paged": (i32, [C.POINTER(AttnPagedArgs), vp]),
     "jb_attn_paged_workspace": (i64, [C.POINTER(AttnPagedArgs)]),
+    "jb_kv_write": (i32, [C.POINTER(KvWriteArgs), vp]),
+    "jb_pages_extend": (i32, [C.POINTER(PageTable), vp, i32, vp, vp, vp, vp]),
+    "jb_pages_free": (i32, [C.POINTER(PageTable), vp, i32, vp, vp]),
+    "jb_pages_fork": (i32, [C.POINTER(PageTable), C.POINTER(PagePools), vp, vp, i32, vp, vp, vp]),
+    "jb_pages_compact": (i32, [C.POINTER(PageTable), C.POINTER(PagePools), vp, vp, vp, vp]),
+    "jb_pages_copy": (i32, [C.POINTER(PagePools), vp, vp, i32, vp]),
+    "jb_sample_filtered": (i32, [C.POINTER(SampleFilteredArgs), vp]),
     "jb_embed": (i32, [i32, vp, vp, i64, vp, vp, vp, i64, vp, i64, i64, i32, i32, i32, vp, i32, vp]),
     "jb_final_add": (i32, [i32, vp, vp, i64, vp, i64, i64, i32, i32, i32, vp, i32, vp]),
     "jb_sample_logits": (i32, [vp, i32, i32, vp, vp, i64, vp, vp, i64, vp]),

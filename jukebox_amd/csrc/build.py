@@ -10,7 +10,7 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = ["api.hip", "gemm.hip", "attention.hip", "elementwise.hip", "engine.hip", "paged_attention.hip"]
+SOURCES = ["api.hip", "gemm.hip", "attention.hip", "elementwise.hip", "engine.hip", "paged_attention.hip", "pages.hip", "sampler.hip"]
 # packed fp32 arithmetic (v_pk_add / mul / fma_f32) stays off: hipcc makes it by itself from ordinary float code, and some of its
 # forms have given wrong results on this hardware now and then, without an error
 FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

@@ -387,6 +387,116 @@ def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, fun
     return out
 
 
+def kv_write(k, v, kpool, vpool, slots):
+    """New key / value rows into pages (jb_kv_write): k, v (n_tokens, n_kv_head, d_head) to the cache rows slots (n_tokens,
+    int64: page * page_size + row in the page; pages_extend makes them) of kpool, vpool (n_pages, page_size, n_kv_head, d_head).
+    Rows whose slot is -1 are left out."""
+    code = _paged_type(k, v, kpool, vpool)
+    _chk_paged(k, v, kpool, vpool, slots)
+    if k.dim() != 3 or kpool.dim() != 4 or k.shape != v.shape or kpool.shape != vpool.shape or k.shape[1:] != kpool.shape[2:]:
+        raise L.JukeboxHipError("expected k, v (n_tokens, n_kv_head, d_head) and kpool, vpool (n_pages, page_size, n_kv_head, d_head)")
+    if k.stride() != v.stride() or kpool.stride() != vpool.stride() or k.stride(2) != 1 or kpool.stride(3) != 1:
+        raise L.JukeboxHipError("expected equal strides of k and v and of kpool and vpool, and contiguous channels")
+    T, KV, D = k.shape
+    if slots.dtype != torch.int64 or slots.shape != (T,) or not slots.is_contiguous():
+        raise L.JukeboxHipError("slots: expected a contiguous int64 array with an entry per token")
+    ts, hs = k.stride()[:2]
+    ps, rs, phs = kpool.stride()[:3]
+    if KV == 1:         # a single head's stride is anything
+        hs = phs = D
+    a = L.KvWriteArgs(code, k.data_ptr(), v.data_ptr(), ts, hs, kpool.data_ptr(), vpool.data_ptr(), ps, rs, phs, kpool.shape[0],
+                      kpool.shape[1], slots.data_ptr(), T, KV, D)
+    _launch(L.lib().jb_kv_write, k.device, C.byref(a))
+
+
+def _page_table(table, lens, ref, page_size, status=None):
+    stride = _chk_table(table)
+    n = table.shape[0]
+    if lens is not None:
+        _chk_int("lens", lens, n)
+    _chk_int("ref", ref, None)
+    if status is not None:
+        _chk_int("status", status, 1)
+    _chk_paged(table, lens, ref, status)
+    return L.PageTable(table.data_ptr(), stride, n, table.shape[1], L.ptr(lens), ref.data_ptr(), ref.shape[0], page_size)
+
+
+def _page_pools(pools, n_pages, device):
+    """Pools of equal shape and strides, (n_pages, ...) with contiguous pages; any type."""
+    if len(pools) == 0:
+        return L.PagePools(None, 0, n_pages, 1, 1)
+    p = pools[0]
+    shape, stride, size = p.shape, p.stride(), p.element_size()
+    n = 1
+    for m, st in zip(reversed(shape[1:]), reversed(stride[1:])):
+        if m > 1 and st != n:
+            raise L.JukeboxHipError("pools: expected contiguous pages")
+        n *= m
+    if shape[0] != n_pages or n == 0 or (n_pages > 1 and stride[0] < n):
+        raise L.JukeboxHipError(f"pools: expected {n_pages} pages that do not overlap")
+    for x in pools:
+        if x.shape != shape or x.stride() != stride or x.element_size() != size or x.device != device:
+            raise L.JukeboxHipError("pools: expected equal shapes, strides and types on the table's GPU")
+    base = (L.vp * len(pools))(*[x.data_ptr() for x in pools])
+    return L.PagePools(base, len(pools), n_pages, n * size, (stride[0] if n_pages > 1 else n) * size)
+
+
+def pages_extend(table, lens, ref, cu_new, page_size, n_tokens, status):
+    """Room for cu_new[i + 1] - cu_new[i] more tokens of every sequence (jb_pages_extend): takes free pages from the lowest on,
+    adds to lens, and returns the cache row of each of the n_tokens new tokens (int64; -1 behind the last).  Without enough free
+    pages nothing changes, all slots are -1 and status (one int32, which the caller clears) says so."""
+    t = _page_table(table, lens, ref, page_size, status)
+    _chk_int("cu_new", cu_new, t.n_seq + 1)
+    _chk_paged(table, cu_new)
+    slots = torch.empty(n_tokens, dtype=torch.int64, device=table.device)
+    work = torch.empty(1 + 2 * t.n_seq + t.n_pages, dtype=torch.int32, device=table.device)
+    _launch(L.lib().jb_pages_extend, table.device, C.byref(t), cu_new.data_ptr(), n_tokens, slots.data_ptr(), work.data_ptr(), status.data_ptr())
+    return slots
+
+
+def pages_free(table, lens, ref, rows, status):
+    """The sequences in these rows (int32) of the table end (jb_pages_free): references given back, rows -1, lengths 0."""
+    t = _page_table(table, lens, ref, 1, status)
+    _chk_int("rows", rows, None)
+    _chk_paged(table, rows)
+    _launch(L.lib().jb_pages_free, table.device, C.byref(t), rows.data_ptr(), rows.shape[0], status.data_ptr())
+
+
+def pages_fork(pools, table, lens, ref, src, dst, page_size, status):
+    """Row dst[i] of the table becomes a fork of row src[i] (jb_pages_fork): shares the full pages and gets a copy of the last,
+    part-filled one in every pool.  pools: a list of (n_pages, ...) tensors -- every layer's keys and values -- with contiguous
+    pages.  The rows dst are empty before (pages_free), and no source."""
+    t = _page_table(table, lens, ref, page_size, status)
+    p = _page_pools(pools, t.n_pages, table.device)
+    _chk_int("src", src, None)
+    _chk_int("dst", dst, src.shape[0])
+    _chk_paged(table, src, dst)
+    work = torch.empty(2 + 4 * src.shape[0], dtype=torch.int32, device=table.device)
+    _launch(L.lib().jb_pages_fork, table.device, C.byref(t), C.byref(p), src.data_ptr(), dst.data_ptr(), src.shape[0], work.data_ptr(), status.data_ptr())
+
+
+def pages_compact(pools, table, ref):
+    """Live pages (ref > 0) moved to the lowest numbers in every pool (jb_pages_compact).  Returns the table and the reference
+    counts that go with the moved pages; the ones given stay as they are."""
+    t = _page_table(table, None, ref, 1)
+    p = _page_pools(pools, t.n_pages, table.device)
+    table_out, ref_out = torch.empty(table.shape, dtype=torch.int32, device=table.device), torch.empty_like(ref)
+    work = torch.empty(2 + 3 * t.n_pages, dtype=torch.int32, device=table.device)
+    _launch(L.lib().jb_pages_compact, table.device, C.byref(t), C.byref(p), table_out.data_ptr(), ref_out.data_ptr(), work.data_ptr())
+    return table_out, ref_out
+
+
+def pages_copy(pools, src, dst):
+    """Page src[i] of every pool to page dst[i] (jb_pages_copy; int32 arrays).  No target twice, no target that is a source."""
+    if len(pools) == 0:
+        return
+    p = _page_pools(pools, pools[0].shape[0], pools[0].device)
+    _chk_int("src", src, None)
+    _chk_int("dst", dst, src.shape[0])
+    _chk_paged(pools[0], src, dst)
+    _launch(L.lib().jb_pages_copy, src.device, C.byref(p), src.data_ptr(), dst.data_ptr(), src.shape[0])
+
+
 def vq_gather(codes, codebook):
     """(N, T) int64 -> (N, T, emb) fp32 (BottleneckBlock.decode, channels-last)."""
     _chk_cuda(codes, codebook)
@@ -416,3 +526,37 @@ def make_sample_params(temp=1.0, top_k=0, top_p=0.0, seed=0, sample_base=0, pos_
     p = L.SampleParams(temp, top_k, top_p, sample_base, seed & 0xFFFFFFFFFFFFFFFF, pos_base, stream_id)
     raw = bytes(p)
     return torch.frombuffer(bytearray(raw), dtype=torch.uint8).to(device)
+
+
+def sample_filtered(logits, u, temp=1.0, top_k=0, top_p=0.0, min_p=0.0, out=None):
+    """One token a row (int64) from given uniform numbers after temperature, top-k, top-p and min-p (jb_sample_filtered has the
+    definition, which the answer equals whatever the sizes).  logits (rows, bins), float32, float16 or bfloat16, rows of any
+    pitch; u (rows) float32 in [0, 1).  temp, top_k, top_p, min_p: a number for all rows or an array with one for each (int32 for
+    top_k, float32 for the others).  temp <= 0: the largest logit; top_k <= 0, top_p <= 0 or >= 1, min_p <= 0: off.  -inf and NaN
+    are forbidden tokens; a row without any other gives -1."""
+    code = _paged_type(logits)
+    if logits.dim() != 2 or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise L.JukeboxHipError("logits: expected rows of contiguous values")
+    n, bins = logits.shape
+    if out is None:
+        out = torch.empty(n, dtype=torch.int64, device=logits.device)
+    elif out.dtype != torch.int64 or out.shape != (n,) or not out.is_contiguous():
+        raise L.JukeboxHipError("out: expected a contiguous int64 array with an entry per row")
+    ptrs, vals, each = [], [], []
+    for name, x, dtype in (("u", u, torch.float32), ("temp", temp, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                           ("min_p", min_p, torch.float32)):
+        if torch.is_tensor(x):
+            if x.dtype != dtype or x.shape != (n,) or not x.is_contiguous():
+                raise L.JukeboxHipError(f"{name}: expected a contiguous {dtype} array with an entry per row")
+            ptrs.append(x.data_ptr())
+            vals.append(0)
+            each.append(x)
+        elif name == "u":
+            raise L.JukeboxHipError("u: expected an array with a uniform number per row")
+        else:
+            ptrs.append(None)
+            vals.append(x)
+    _chk_paged(logits, out, *each)
+    a = L.SampleFilteredArgs(code, logits.data_ptr(), logits.stride(0) if n > 1 else bins, n, bins, *ptrs, *vals[1:], out.data_ptr())
+    _launch(L.lib().jb_sample_filtered, logits.device, C.byref(a))
+    return out
