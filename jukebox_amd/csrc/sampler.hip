@@ -13,13 +13,27 @@
 
 namespace {
 
-constexpr int NT = 1024, NB = 2048, CAP = 1024;       // threads of a row; histogram bins; entries of the exact selection
+constexpr int NB = 2048, CAP = 1024;                  // histogram bins; entries of the exact selection
 constexpr double W1 = 17592186044416.0;               // 2^44: the weight of the largest logit
 constexpr double RANGE = 32.0;                        // exp(-31.98) 2^44 < 0.5: entries further from the largest weigh nothing
 constexpr int MAX_BINS = 1 << 18;
-constexpr double LN2_REST = 1.908214929270587816e-10;   // ln 2 - 2977044471 / 2^32
 
 typedef unsigned long long u64;
+
+// 2^(j / 32): correctly rounded, from 50 decimal digits
+__constant__ double EXP2_32[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+
+// (ln 2 / 32)^k / k!
+constexpr double LN2_32 = 0.69314718055994530942 / 32.0;
+constexpr double L1 = LN2_32, L2 = LN2_32 * LN2_32 / 2.0, L3 = LN2_32 * LN2_32 * LN2_32 / 6.0, L4 = LN2_32 * LN2_32 * LN2_32 * LN2_32 / 24.0;
 
 template <typename T> struct Row;                     // 16 bytes of logits at a time
 template <> struct Row<float> { static constexpr int E = 4; static __device__ __forceinline__ float get(u32x4 v, int e) { return __uint_as_float(v[e]); } };
@@ -31,56 +45,84 @@ template <> struct Row<bf16> {
     static constexpr int E = 8;
     static __device__ __forceinline__ float get(u32x4 v, int e) { return __uint_as_float((e & 1) ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16); }
 };
-// NaN counts as a forbidden token; -0 is 0
-__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
-// E logits from index i on; -inf behind the row's end
-template <typename T> __device__ __forceinline__ void load_row(const T* row, int i, int n, float (&x)[Row<T>::E]) {
+// E logits from index i on; -inf behind the row's end.  A NaN may come out: fmaxf and the bins pass it over.
+template <typename T> __device__ __forceinline__ u32x4 load_row(const T* row, int i, int n) {
     constexpr int E = Row<T>::E;
-    if (i + E <= n) {
-        const u32x4 v = *reinterpret_cast<const u32x4_any*>(row + i);
+    if (i + E <= n) return *reinterpret_cast<const u32x4_any*>(row + i);
+    u32x4 v;
+    if constexpr (E == 4) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = clean(Row<T>::get(v, e));
+        for (int e = 0; e < 4; ++e) v[e] = i + e < n ? __float_as_uint(row[i + e]) : 0xff800000u;
     } else {
+        const unsigned none = sizeof(T) == 2 && __is_same(T, f16) ? 0xfc00u : 0xff80u;
+        const unsigned short* bits = reinterpret_cast<const unsigned short*>(row);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = i + e < n ? clean((float)row[i + e]) : -INFINITY;
+        for (int h = 0; h < 4; ++h)
+            v[h] = (i + 2 * h < n ? bits[i + 2 * h] : none) | (i + 2 * h + 1 < n ? bits[i + 2 * h + 1] : none) << 16;
+    }
+    return v;
+}
+// f(logit, index) for the whole row, every thread its part: U 16-byte requests in flight
+template <typename T, int NT, typename F> __device__ __forceinline__ void each(const T* row, int n, F f) {
+    constexpr int E = Row<T>::E, STEP = NT * E, U = 16 / E;
+    for (int i = threadIdx.x * E; i < n; i += U * STEP) {
+        u32x4 v[U];
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+            if (i + q * STEP < n) v[q] = load_row(row, i + q * STEP, n);
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+            if (i + q * STEP < n) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) f(Row<T>::get(v[q], e), i + q * STEP + e);
+            }
     }
 }
 
-// exp(y) for y <= 0: y = n ln 2 + r, |r| <= ln 2 / 2, exp(r) by its Taylor series to r^13 (the next term: 2^-54).
-// Coefficients 1 / k!.
-__device__ __forceinline__ double exp_neg(double y) {
-    const double n = rint(y * 1.4426950408889634074);
-    double r = fma(n, -2977044471.0 / 4294967296.0, y);          // ln 2 = its first 32 bits and the rest: n times the first is exact
-    r = fma(n, -LN2_REST, r);
-    double p = 1.0 / 6227020800.0;
-    p = fma(p, r, 1.0 / 479001600.0);
-    p = fma(p, r, 1.0 / 39916800.0);
-    p = fma(p, r, 1.0 / 3628800.0);
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return ldexp(p, (int)n);
-}
+// order-preserving integers of floats
+__device__ __forceinline__ unsigned key_of(float x) { const unsigned b = __float_as_uint(x); return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u); }
+__device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
+
 struct Weigh {
     float mx, bins;                                   // largest logit; bins per unit of logit
-    double inv_t, min_p;
-    // entries further below the largest than RANGE temperatures are in the last bin and weigh nothing
-    __device__ __forceinline__ int bin(float x) const { return x == mx ? 0 : (int)fminf((mx - x) * bins, (float)(NB - 1)); }
-    __device__ __forceinline__ double real(float x) const { return x == mx ? 1.0 : exp_neg(((double)x - (double)mx) * inv_t); }
+    double c, md;                                     // 32 / (T ln 2); the largest logit
+    const double* tab;                                // EXP2_32 in LDS: 32 entries, one pair of banks each
+    // how far below the largest, in bins; NB - 1: weighs nothing
+    __device__ __forceinline__ float depth(float x) const { return x == mx ? 0.f : fminf((mx - x) * bins, (float)(NB - 1)); }
+    __device__ __forceinline__ int bin(float x) const { return (int)depth(x); }
+    // The largest x that lies in bin b or below it (depth falls with x, also as it is rounded), so that telling an entry's bin takes
+    // comparisons alone.  The whole wave: its lanes divide the interval by 64 at a time.
+    __device__ __forceinline__ float below(int b) const {
+        if (b == 0) return INFINITY;
+        unsigned lo = key_of(-INFINITY), hi = key_of(mx);          // depth(lo) >= b > depth(hi)
+        while (hi - lo > 1) {
+            const unsigned step = (hi - lo + 63) / 64, m = min(lo + step * ((threadIdx.x & 63) + 1), hi);
+            const int n = __popcll(__ballot(m < hi && depth(of_key(m)) >= (float)b));      // the first n lanes
+            lo += step * n;
+            hi = min(lo + step, hi);
+        }
+        return of_key(lo);
+    }
+    // 2^44 exp((x - max) / T) in double: z = n + f in 32nds of an octave; 2^(f / 32) by the Taylor series of the exponential to the
+    // fourth power (f <= 1/2: the next term is 1.2e-12 of the weight), 2^(n / 32) from the table and the exponent field.  n by
+    // adding and taking away 1.5 2^52, in whose low word it stands meanwhile.  For x within RANGE T of the largest.
+    __device__ __forceinline__ double real(float x) const {
+        const double z = x == mx ? 0.0 : ((double)x - md) * c, t = z + 6755399441055744.0, f = z - (t - 6755399441055744.0);
+        double p = fma(f, L4, L3);
+        p = fma(p, f, L2);
+        p = fma(p, f, L1);
+        p = fma(p, f, 1.0);
+        const int n = (int)__double_as_longlong(t);
+        const double w = p * tab[n & 31];
+        return __hiloint2double(__double2hiint(w) + ((n >> 5) + 44) * 0x100000, __double2loint(w));
+    }
     // a whole number in the low bits of the sum with 2^52: rounded to nearest
-    static __device__ __forceinline__ u64 whole(double w) { return (u64)__double_as_longlong(w * W1 + 4503599627370496.0) & 0xfffffffffffffull; }
+    static __device__ __forceinline__ u64 whole(double w) { return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull; }
+    __device__ __forceinline__ u64 whole(float x) const { return whole(real(x)); }
 };
-// order (x descending, index ascending) as one ascending integer
+// order (x descending, index ascending) as one ascending integer; -0 counts as 0
 __device__ __forceinline__ u64 place(float x, int i) {
-    const unsigned b = __float_as_uint(x), up = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-    return ((u64)~up << 32) | (unsigned)i;
+    return ((u64)~key_of(x + 0.0f) << 32) | (unsigned)i;
 }
 
 __device__ __forceinline__ u64 wave_sum(u64 v) {
@@ -102,15 +144,16 @@ struct Shared {
     unsigned count[NB];
     u64 at[CAP];                                      // the border bin's entries: their places ...
     u64 w[CAP];                                       // ... and weights
-    u64 tile[MAX_BINS / 256];                         // kept weight of 64 E consecutive entries
-    u64 part[NT / 64];
-    float fpart[NT / 64];
+    u64 tile[MAX_BINS / 1024];                        // kept weight of 256 E consecutive entries
+    double tab[32];
+    u64 part[16];
     u64 border;                                       // place of the last kept entry
-    u64 before_w; unsigned before_n, n;               // of the border bin; entries listed
+    u64 before_w, before_n;                           // in front of the bin that a search has found
+    unsigned n;                                       // entries listed
     int pick;
 };
 // inclusive prefix sum over the block; *total: all
-__device__ __forceinline__ u64 block_scan(u64 v, Shared& s, u64* total) {
+template <int NT> __device__ __forceinline__ u64 block_scan(u64 v, Shared& s, u64* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const u64 x = wave_scan(v);
     if (lane == 63) s.part[wave] = x;
@@ -130,208 +173,321 @@ struct Args {
     int64_t* out;
 };
 
-// The first bin at which the running sum of `v` (two bins a thread, in order) exceeds `limit`; NB if none does.  s.before_*: the
-// sums in front of it.
-template <typename V> __device__ int crossing(const V* v, u64 limit, Shared& s, u64* before) {
-    if (threadIdx.x == 0) { s.pick = NB; s.before_w = 0; }
+template <int NT> __device__ __forceinline__ void clear_bins(Shared& s) {
+    for (int i = threadIdx.x; i < NB; i += NT) { s.mass[i] = 0; s.count[i] = 0; }
     __syncthreads();
-    const u64 a = v[2 * threadIdx.x], b = v[2 * threadIdx.x + 1];
-    u64 total;
-    const u64 inc = block_scan(a + b, s, &total), exc = inc - a - b;
-    if (exc <= limit && inc > limit) {
-        const bool second = exc + a <= limit;
-        s.pick = 2 * threadIdx.x + second;
-        s.before_w = exc + (second ? a : 0);
+}
+// f(logit) is true for the entries that count: add(bin, weight) for each.  Where a whole wave's 16 bytes hold one value (a mask's, over
+// half the vocabulary), whose additions would queue up at one address, it enters once, for all of them.
+template <typename T, int NT, typename F> __device__ __forceinline__ void each_run(const T* row, int n, F f) {
+    constexpr int E = Row<T>::E, STEP = NT * E, U = 16 / E;
+    for (int i = threadIdx.x * E; i < n; i += U * STEP) {
+        u32x4 v[U];
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+            if (i + q * STEP < n) v[q] = load_row(row, i + q * STEP, n);
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+            if (i + q * STEP >= n) continue;
+            const unsigned w = v[q][0], one = __builtin_amdgcn_readfirstlane(w);
+            const bool same = w == one && v[q][1] == one && v[q][2] == one && v[q][3] == one && (E == 4 || (one >> 16) == (one & 0xffffu));
+            const u64 all = __ballot(1);
+            if (__ballot(same) == all) {
+                if ((all & ((1ull << (threadIdx.x & 63)) - 1)) == 0) f(Row<T>::get(v[q], 0), (unsigned)__popcll(all) * E);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) f(Row<T>::get(v[q], e), 1u);
+            }
+        }
+    }
+}
+// The first bin at which the running count (COUNT) or weight exceeds `limit`; NB if none does.  s.before_*: the sums in front of it.
+template <int NT, bool COUNT> __device__ int crossing(u64 limit, Shared& s, bool weights_too = false) {
+    constexpr int PER = NB / NT;
+    if (threadIdx.x == 0) s.pick = NB;
+    __syncthreads();
+    u64 c = 0, w = 0, total;
+#pragma unroll
+    for (int b = 0; b < PER; ++b) {
+        if (COUNT) c += s.count[PER * threadIdx.x + b];
+        if (!COUNT || weights_too) w += s.mass[PER * threadIdx.x + b];
+    }
+    u64 ic = COUNT ? block_scan<NT>(c, s, &total) - c : 0, iw = !COUNT || weights_too ? block_scan<NT>(w, s, &total) - w : 0;
+    if ((COUNT ? ic : iw) <= limit && (COUNT ? ic + c : iw + w) > limit) {
+        for (int b = PER * threadIdx.x; ; ++b) {
+            const u64 nc = ic + (COUNT ? s.count[b] : 0), nw = iw + (!COUNT || weights_too ? s.mass[b] : 0);
+            if ((COUNT ? nc : nw) > limit) { s.pick = b; s.before_n = ic; s.before_w = iw; break; }
+            ic = nc; iw = nw;
+        }
     }
     __syncthreads();
-    const int r = s.pick;
-    *before = s.before_w;
-    __syncthreads();
-    return r;
+    return s.pick;
 }
 
-template <typename T>
+// The last kept entry of a bin -- COUNT: the `limit`-th after its first; else the last one that no more than `limit` of weight is
+// before -- and the bin's weight up to and with it.
+struct Found { u64 border, mass; };
+
+// Many entries in the bin (equal logits): by the digits of their places, which are all different.  Rare, hence a call.
+template <typename T, int NT, bool COUNT>
+__device__ __attribute__((noinline)) Found search_digits(const T* row, int n, const Weigh g, int which, u64 limit, bool with_mass, Shared& s) {
+    const float lo = g.below(which + 1), hi = g.below(which);
+    u64 prefix = 0, before = 0;
+    for (int d = 0; d < 5; ++d) {
+        __syncthreads();
+        clear_bins<NT>(s);
+        // 32 bits of the logit as 11, 11 and 10, 18 of the index as 9 and 9
+        const int bits = d < 2 ? 11 : d == 2 ? 10 : 9, sh = d < 3 ? 64 - 11 * d - bits : 9 * (4 - d), top = sh + bits;
+        auto add = [&](float x, int i, unsigned times) {
+            if (x > lo && x <= hi) {
+                const u64 p = place(x, i);
+                if (d == 0 || (p ^ prefix) >> (top & 63) == 0) {
+                    const int b = (int)(p >> sh) & ((1 << bits) - 1);
+                    if (COUNT) atomicAdd(&s.count[b], times);
+                    if (with_mass || !COUNT) atomicAdd(&s.mass[b], g.whole(x) * times);
+                }
+            }
+        };
+        if (d < 3) each_run<T, NT>(row, n, [&](float x, unsigned times) { add(x, 0, times); });
+        else each<T, NT>(row, n, [&](float x, int i) { add(x, i, 1u); });
+        __syncthreads();
+        const int b = crossing<NT, COUNT>(limit, s, with_mass);
+        // (none: everything of this prefix is kept -- its largest place stands for it)
+        if (b == NB) { prefix |= d == 0 ? ~0ull : (1ull << top) - 1; break; }
+        prefix |= (u64)b << sh;
+        limit -= COUNT ? s.before_n : s.before_w;
+        before += s.before_w;
+        if (d == 4) before += s.mass[b];
+    }
+    __syncthreads();
+    return Found{prefix, before};
+}
+template <typename T, int NT, bool COUNT>
+__device__ __forceinline__ Found select(const T* row, int n, const Weigh& g, int which, u64 limit, bool with_mass, Shared& s) {
+    if (threadIdx.x == 0) { s.n = 0; s.border = 0; }
+    __syncthreads();
+    const float lo = g.below(which + 1), hi = g.below(which);       // the bin's logits: lo < x <= hi
+    each<T, NT>(row, n, [&](float x, int i) {
+        if (x > lo && x <= hi) {
+            const unsigned at = atomicAdd(&s.n, 1u);
+            if (at < CAP) { s.at[at] = place(x, i); s.w[at] = g.whole(x); }
+        }
+    });
+    __syncthreads();
+    const unsigned m = s.n;
+    if (m > CAP) return search_digits<T, NT, COUNT>(row, n, g, which, limit, with_mass, s);
+    // entry against entry
+    u64 sum = 0;
+    for (unsigned t = threadIdx.x; t < m; t += NT) {
+        const u64 me = s.at[t];
+        unsigned nb = 0;
+        u64 wb = 0;
+        if (COUNT) {
+#pragma unroll 8
+            for (unsigned j = 0; j < m; ++j) nb += s.at[j] < me;
+        } else {
+#pragma unroll 4
+            for (unsigned j = 0; j < m; ++j) wb += s.at[j] < me ? s.w[j] : 0;
+        }
+        if ((COUNT ? nb : wb) <= limit) { atomicMax(&s.border, me); sum += s.w[t]; }
+    }
+    Found f;
+    block_scan<NT>(sum, s, &f.mass);
+    f.border = s.border;
+    return f;
+}
+
+template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_filtered_kernel(const Args a) {
-    constexpr int E = Row<T>::E, STEP = NT * E;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    Shared& s = *reinterpret_cast<Shared*>(smem);
+    constexpr int E = Row<T>::E;
+    __shared__ Shared s;
     const int n = a.bins, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r = blockIdx.x;
     const T* row = (const T*)a.logits + r * a.ld;
-    float x[E];
 
-    // ---- the largest logit and its first index ---------------------------------------------------------------------------------
-    u64 first = ~0ull;
-    for (int i = tid * E; i < n; i += STEP) {
-        load_row(row, i, n, x);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (i + e < n) { const u64 p = place(x[e], i + e); first = p < first ? p : first; }
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { const u64 u = __shfl_xor(first, o); first = u < first ? u : first; }
-    if (lane == 0) s.part[wave] = first;
+    // ---- the largest logit --------------------------------------------------------------------------------------------------------
+    float top = -INFINITY;
+    each<T, NT>(row, n, [&](float x, int) { top = fmaxf(top, x); });
+    top = jb_wave_max(top);
+    if (lane == 0) s.part[wave] = __float_as_uint(top);
+    if (tid < 32) s.tab[tid] = EXP2_32[tid];
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) first = s.part[w] < first ? s.part[w] : first;
+    for (int w = 0; w < NT / 64; ++w) top = fmaxf(top, __uint_as_float((unsigned)s.part[w]));
     __syncthreads();
-    const unsigned up = ~(unsigned)(first >> 32);
-    const float mx = __uint_as_float(up ^ ((up >> 31) ? 0x80000000u : 0xffffffffu));
     const float temp = a.temp ? a.temp[r] : a.temp_all;
-    if (mx == -INFINITY || !(temp > 0.f)) {           // nothing allowed: -1; temperature 0: the largest
-        if (tid == 0) a.out[r] = mx == -INFINITY ? -1 : (int64_t)(unsigned)first;
+    if (top == -INFINITY || !(temp > 0.f)) {          // nothing allowed: -1; temperature 0: the largest
+        if (tid == 0) s.pick = 0x7fffffff;
+        __syncthreads();
+        if (top > -INFINITY) each<T, NT>(row, n, [&](float x, int i) { if (x == top) atomicMin(&s.pick, i); });
+        __syncthreads();
+        if (tid == 0) a.out[r] = top > -INFINITY ? s.pick : -1;
         return;
     }
     const int k = a.top_k ? a.top_k[r] : a.top_k_all;
     const float p = a.top_p ? a.top_p[r] : a.top_p_all;
     Weigh g;
-    g.mx = mx; g.inv_t = 1.0 / (double)temp; g.bins = (float)((double)NB / RANGE * g.inv_t); g.min_p = fmin((double)(a.min_p ? a.min_p[r] : a.min_p_all), 1.0);
+    g.mx = top;
+    g.c = 1.0 / (LN2_32 * (double)temp);
+    g.md = (double)g.mx;
+    g.bins = (float)fmin((double)NB / RANGE / (double)temp, 1e30);
+    g.tab = s.tab;
+    const double least = fmin((double)(a.min_p ? a.min_p[r] : a.min_p_all), 1.0) * W1;
     const bool by_k = k > 0 && k < n, by_p = p > 0.f && p < 1.f;
     u64 border = ~0ull;
+    // entries up to this logit weigh nothing.  (Of a row whose largest logit is infinite only its equals weigh anything.)
+    const float zero = g.below(NB - 1);
 
     if (by_k || by_p) {
-        for (int i = tid; i < NB; i += NT) { s.mass[i] = 0; s.count[i] = 0; }
+        clear_bins<NT>(s);
+        each_run<T, NT>(row, n, [&](float x, unsigned times) {
+            if (x > zero) {
+                const int b = g.bin(x);
+                if (by_k) atomicAdd(&s.count[b], times);
+                if (by_p) atomicAdd(&s.mass[b], g.whole(x) * times);
+            }
+        });
         __syncthreads();
-        for (int i = tid * E; i < n; i += STEP) {
-            load_row(row, i, n, x);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int b = g.bin(x[e]);
-                if (b < NB - 1) {
-                    if (by_k) atomicAdd(&s.count[b], 1u);
-                    if (by_p) atomicAdd(&s.mass[b], Weigh::whole(g.real(x[e])));
-                }
-            }
-        }
-        __syncthreads();
-        u64 before_n = 0, before_w = 0, limit_w = ~0ull;
-        int bin = NB;
-        // Entries of one bin in exact order: for each, what of its bin comes before it.
-        auto list_bin = [&](int which) {
-            if (tid == 0) s.n = 0;
+        int kb = NB;
+        u64 total = 0, limit = 0, before = 0;
+        int pb = NB;
+        if (by_p) {                                   // (before the histogram is used up by a search)
+            u64 all, mine = 0;
+            if (by_k) kb = crossing<NT, true>((u64)k - 1, s);
+            const u64 before_n = by_k ? s.before_n : 0;
             __syncthreads();
-            for (int i = tid * E; i < n; i += STEP) {
-                load_row(row, i, n, x);
+            constexpr int PER = NB / NT;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (g.bin(x[e]) == which && i + e < n && x[e] > -INFINITY) {
-                        const unsigned at = atomicAdd(&s.n, 1u);
-                        if (at < CAP) { s.at[at] = place(x[e], i + e); s.w[at] = Weigh::whole(g.real(x[e])); }
-                    }
-            }
-            __syncthreads();
-        };
-        // The last kept entry among those of bin `which` whose place is at most `upto`: rank below `rank` and weight before within `limit`.
-        // Bins of up to CAP entries are ranked entry against entry; larger ones (many equal logits) are halved by place, 64 times.
-        auto select = [&](int which, u64 rank, u64 limit, u64 upto, u64* mass) {
-            list_bin(which);
-            const unsigned m = s.n;
-            if (tid == 0) s.border = 0;
-            __syncthreads();
-            u64 sum = 0;
-            if (m <= CAP) {
-                if (tid < m && s.at[tid] <= upto) {
-                    const u64 me = s.at[tid];
-                    u64 nb = 0, wb = 0;
-                    for (unsigned j = 0; j < m; ++j)
-                        if (s.at[j] < me) { ++nb; wb += s.w[j]; }
-                    if (nb < rank && wb <= limit) { atomicMax(&s.border, me); sum = s.w[tid]; }
-                }
-                u64 total;
-                block_scan(sum, s, &total);
-                *mass = total;
-                return s.border;
-            }
-            // the largest place L with  #{place < L} < rank  and  weight{place < L} <= limit  among places <= upto: by bisection
-            auto below = [&](u64 L, u64* cnt, u64* wt) {
-                u64 c = 0, w = 0;
-                for (int i = tid * E; i < n; i += STEP) {
-                    load_row(row, i, n, x);
+            for (int b = PER * tid; b < PER * (tid + 1); ++b) mine += b < kb ? s.mass[b] : 0;
+            block_scan<NT>(mine, s, &all);
+            total = all;
+            u64 part = 0;
+            if (kb < NB) {
+                // the histogram is needed again after the selection, which may clear it: keep this thread's bins
+                u64 keep_m[PER];
 #pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (i + e < n && x[e] > -INFINITY && g.bin(x[e]) == which && place(x[e], i + e) < L) { ++c; w += Weigh::whole(g.real(x[e])); }
-                }
-                block_scan(c, s, cnt);
-                block_scan(w, s, wt);
-            };
-            u64 L = 0, c, w;
-            for (int bit = 63; bit >= 0; --bit) {
-                const u64 cand = L | (1ull << bit);
-                below(cand, &c, &w);
-                if (c < rank && w <= limit) L = cand;
+                for (int b = 0; b < PER; ++b) keep_m[b] = s.mass[PER * tid + b];
+                const Found f = select<T, NT, true>(row, n, g, kb, (u64)k - 1 - before_n, true, s);
+                border = f.border;
+                part = f.mass;
+                __syncthreads();
+#pragma unroll
+                for (int b = 0; b < PER; ++b) s.mass[PER * tid + b] = keep_m[b];
+                __syncthreads();
             }
-            // L: the largest value for which the entries before it still leave room: every entry at or before L is kept
-            if (L > upto) L = upto;
-            below(L + (L != ~0ull), &c, &w);
-            *mass = w;
-            return L;
-        };
-        u64 mass_k = 0;
-        if (by_k) {
-            bin = crossing(s.count, (u64)k - 1, s, &before_n);
-            if (bin < NB) {
-                border = select(bin, (u64)k - before_n, ~0ull, ~0ull, &mass_k);
-            }
-        }
-        if (by_p) {
-            // weight of what top-k has left: the bins before its border's, and the border bin's part
-            u64 total, all;
-            u64 mine = 0;
-            for (int b = 2 * tid; b < 2 * tid + 2; ++b) mine += b < bin ? s.mass[b] : 0;
-            block_scan(mine, s, &all);
-            total = all + (bin < NB ? mass_k : 0);
             // before <= p total, in whole numbers
-            limit_w = (u64)((double)p * (double)total);
-            const int pb = crossing(s.mass, limit_w, s, &before_w);
-            if (pb < bin || (pb == bin && bin < NB)) border = select(pb, ~0ull, limit_w - before_w, border, &mass_k);
+            limit = (u64)((double)p * (double)(total + part));
+            pb = crossing<NT, false>(limit, s);
+            before = s.before_w;
+            __syncthreads();
+            if (pb < kb || (pb == kb && kb < NB)) {
+                const Found f = select<T, NT, false>(row, n, g, pb, limit - before, true, s);
+                border = f.border < border ? f.border : border;
+            }
+        } else {
+            kb = crossing<NT, true>((u64)k - 1, s);
+            const u64 before_n = s.before_n;
+            __syncthreads();
+            if (kb < NB) border = select<T, NT, true>(row, n, g, kb, (u64)k - 1 - before_n, false, s).border;
         }
+        __syncthreads();
     }
 
     // ---- the draw: kept weights by index ------------------------------------------------------------------------------------------
-    const int tiles = (n + 64 * E - 1) / (64 * E);
-    auto kept = [&](float v, int i) -> u64 {
-        if (i >= n || g.bin(v) >= NB - 1 || place(v, i) > border) return 0;
-        const double w = g.real(v);
-        return w >= g.min_p ? Weigh::whole(w) : 0;
+    constexpr int TILE = 256 * E;
+    const int tiles = (n + TILE - 1) / TILE;
+    // what top-k and top-p have kept: x > cut, or x == cut and index <= last
+    const float cut = border == ~0ull ? zero : of_key(~(unsigned)(border >> 32));
+    const int last = border == ~0ull ? -1 : (int)(unsigned)border;
+    const bool few = border != ~0ull || least > 0.0;
+    // (a little below what min-p leaves, in logits: the weight itself decides)
+    float rough = zero;
+    if (least > 0.0) {
+        const float f = (float)((double)top + (double)temp * (log(least / W1) - 1e-3)) - fabsf(top) * 0x1p-22f;
+        if (f > zero && f < top) rough = f;
+    }
+    auto in = [&](float x, int i) { return x > rough && (x > cut || (x == cut && i <= last)); };
+    auto weight = [&](float x) -> u64 {
+        const double w = g.real(x);
+        return w >= least ? Weigh::whole(w) : 0;
     };
     for (int t = wave; t < tiles; t += NT / 64) {
-        const int i = t * 64 * E + lane * E;
+        const int i = t * TILE + lane * E;
+        u32x4 v[4];
         u64 w = 0;
-        if (i < n) {
-            load_row(row, i, n, x);
 #pragma unroll
-            for (int e = 0; e < E; ++e) w += kept(x[e], i + e);
+        for (int q = 0; q < 4; ++q)
+            if (i + q * 64 * E < n) v[q] = load_row(row, i + q * 64 * E, n);
+        if (few) {
+            // most tiles of a short list hold nothing of it
+            float most = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (i + q * 64 * E < n) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) most = fmaxf(most, Row<T>::get(v[q], e));
+                }
+            if (__any(most >= cut && most > rough)) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (i + q * 64 * E < n) {
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const float x = Row<T>::get(v[q], e);
+                            if (in(x, i + q * 64 * E + e)) w += weight(x);
+                        }
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (i + q * 64 * E < n) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float x = Row<T>::get(v[q], e);
+                        if (x > zero) w += g.whole(x);
+                    }
+                }
         }
         w = wave_sum(w);
         if (lane == 0) s.tile[t] = w;
     }
     __syncthreads();
-    const int per = (tiles + NT - 1) / NT;
-    u64 mine = 0, total;
-    for (int t = tid * per; t < min(tiles, (tid + 1) * per); ++t) mine += s.tile[t];
-    const u64 inc = block_scan(mine, s, &total);
+    u64 total;
+    const u64 mine = tid < tiles ? s.tile[tid] : 0, inc = block_scan<NT>(mine, s, &total);
     const float uf = a.u[r];
     const double ud = uf > 0.f ? (double)uf : 0.0;                 // NaN and less: the first kept token
     u64 goal = (u64)fmin(ud * (double)total, 9.0e18);
     if (goal >= total) goal = total - 1;                           // 1 and more: the last (the largest logit always weighs something)
-    u64 left = inc - mine;
-    if (left <= goal && inc > goal)
-        for (int t = tid * per; t < min(tiles, (tid + 1) * per); ++t) {
-            if (left + s.tile[t] > goal) { s.pick = t; s.before_w = left; break; }
-            left += s.tile[t];
-        }
+    if (inc - mine <= goal && inc > goal) { s.pick = tid; s.before_w = inc - mine; }
     __syncthreads();
-    if (wave == 0) {
-        const int i = s.pick * 64 * E + lane * E;
-        u64 w[E], sum = 0;
-        if (i < n) load_row(row, i, n, x);
+    // the tile's four parts by four waves, the one whose part it is in by its lanes
+    u64 w[E], sum = 0;
+    const int i = s.pick * TILE + wave * 64 * E + lane * E;
+    if (wave < 4) {
+        if (i < n) {
+            const u32x4 v = load_row(row, i, n);
 #pragma unroll
-        for (int e = 0; e < E; ++e) { w[e] = i < n ? kept(x[e], i + e) : 0; sum += w[e]; }
-        u64 at = s.before_w + wave_scan(sum) - sum;
+            for (int e = 0; e < E; ++e) {
+                const float x = Row<T>::get(v, e);
+                w[e] = in(x, i + e) ? weight(x) : 0;
+                sum += w[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = 0;
+        }
+    }
+    const u64 upto = wave_scan(sum);
+    if (lane == 63) s.part[wave] = upto;
+    __syncthreads();
+    if (wave < 4) {
+        u64 mark = s.before_w + upto - sum;
+        for (int q = 0; q < wave; ++q) mark += s.part[q];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if (at <= goal && at + w[e] > goal) a.out[r] = i + e;
-            at += w[e];
+            if (mark <= goal && mark + w[e] > goal) a.out[r] = i + e;
+            mark += w[e];
         }
     }
 }
@@ -346,11 +502,15 @@ extern "C" int jb_sample_filtered(const jb_sample_filtered_args* a, void* stream
     if (a->rows == 0) return JB_OK;
     JB_REQUIRE(a->logits && a->u && a->tokens, "null pointer");
     const Args k = {a->logits, a->ld, a->bins, a->u, a->temp, a->top_k, a->top_p, a->min_p, a->temp_all, a->top_k_all, a->top_p_all, a->min_p_all, a->tokens};
-    static_assert(sizeof(Shared) <= 64 * 1024, "LDS");
     hipStream_t s = (hipStream_t)stream;
-    if (a->dtype == JB_F32) sample_filtered_kernel<float><<<(unsigned)a->rows, NT, sizeof(Shared), s>>>(k);
-    else if (a->dtype == JB_F16) sample_filtered_kernel<f16><<<(unsigned)a->rows, NT, sizeof(Shared), s>>>(k);
-    else sample_filtered_kernel<bf16><<<(unsigned)a->rows, NT, sizeof(Shared), s>>>(k);
+    // rows of up to 16384 tokens: four waves, whose barriers cost less than the other twelve would save
+#define JB_GO(T)                                                                                   \
+    do {                                                                                           \
+        if (a->bins <= 16384) sample_filtered_kernel<T, 256><<<(unsigned)a->rows, 256, 0, s>>>(k); \
+        else sample_filtered_kernel<T, 1024><<<(unsigned)a->rows, 1024, 0, s>>>(k);                \
+    } while (0)
+    if (a->dtype == JB_F32) JB_GO(float); else if (a->dtype == JB_F16) JB_GO(f16); else JB_GO(bf16);
+#undef JB_GO
     JB_CHECK_LAUNCH();
     return JB_OK;
 }
