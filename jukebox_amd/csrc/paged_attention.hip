@@ -135,27 +135,37 @@ template <typename T> __device__ __forceinline__ void store8(T* o, const float* 
     *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, x);
 }
 
-// One workgroup of four waves per (sequence, kv head, tile of 16 rows, split of the keys); a wave takes every fourth 32-key turn
-// of its split with a running maximum and sum of its own, and the four states join through LDS.
+// One workgroup per (sequence, kv head, tile of 16 rows, split of the keys).
 //
 //   S^T = K Q^T     A = 16 keys x 32 channels straight from the cache rows, B = the rows' queries (in registers throughout): a
 //                   lane holds, for query row l & 15, the scores of keys (l >> 4) * 4 + r of both 16-key halves -- the softmax
 //                   statistics take two cross-lane steps, and the rescaling of the output none.
 //   O^T += V^T P^T  the order of a product's inner index is free: slot (g, i) is key (i / 4) * 16 + g * 4 + i % 4, so the B
 //                   operand is the lane's own probabilities, and the A operand the lane's own eight value pieces (gather above).
-// K and V therefore go from memory to the matrix cores through registers alone: no LDS, no barrier inside the loop.
+// K and V therefore go from memory to the matrix cores through registers alone.
 // In 16 bits the probabilities enter as a high and a low part (two products): the output is as near the 64-bit value as its own
 // rounding allows; the products hide behind the memory anyway (one new token: 1 row of 16 used).
-// NC: chunks of 16 E channels that cover d_head.
+// NC slices of 16 E channels cover d_head, each a wave's: heads of up to 128 halfs have four waves side by side on the keys, every
+// one with a running maximum and sum of its own, joined through LDS at the end; wider heads NC waves to a turn of 32 keys, which add
+// up their parts of the scores through LDS (one barrier a turn).  One wave for a whole head of 480 channels held 512 registers, four
+// waves a compute unit, each request waiting for the one before: 238 us for 16 sequences of 4096-8192 keys, now MEASURED.
+template <typename T, int NC> struct Shape {
+    static constexpr int WAVES = NC > 4 ? NC : 4, KG = WAVES / NC, CH = 16 * El<T>::E, LDO = CH + 4;     // LDO: rows 4 banks apart
+    struct Shared {
+        float s[NC > 1 ? 2 : 1][NC > 1 ? WAVES : 1][NC > 1 ? 64 : 1][8];      // parts of the scores, two turns' worth
+        float o[KG > 1 ? WAVES : 1][KG > 1 ? 16 : 1][LDO];
+        float ml[KG][16][2];
+    };
+};
 template <typename T, int NC>
-__global__ __launch_bounds__(256) void attn_paged_rows_kernel(const Args a) {
+__global__ __launch_bounds__((Shape<T, NC>::WAVES * 64)) void attn_paged_rows_kernel(const Args a) {
     typedef typename El<T>::vec vec;
-    constexpr int E = El<T>::E, CH = 16 * E, KT = 4 * E, NK = NC * CH / KT;
-    constexpr bool WIDE = NC * E > 8;
-    constexpr int LDO = CH + 4;                  // floats between two rows of the exchange: rows 4 banks apart
-    __shared__ float s_o[4][16][LDO];
-    __shared__ float s_ml[4][16][2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    typedef Shape<T, NC> Sh;
+    constexpr int E = El<T>::E, CH = Sh::CH, KT = 4 * E, NK = CH / KT, KG = Sh::KG;
+    __shared__ typename Sh::Shared sh;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    // scalar, so that what depends on the wave branches: matrix instructions run whatever the lanes' mask, also under an empty one
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / NC, cb = wave % NC * CH;
     int64_t b = blockIdx.x;
     const int tile0 = (int)(b % a.tiles); b /= a.tiles;
     const int split = (int)(b % a.splits); b /= a.splits;
@@ -164,7 +174,8 @@ __global__ __launch_bounds__(256) void attn_paged_rows_kernel(const Args a) {
     const int n_tiles = tiles_of(a, s.nq);
     const T* kbase = (const T*)a.k + (int64_t)kvh * a.head_stride;
     const T* vbase = (const T*)a.v + (int64_t)kvh * a.head_stride;
-    const int D = a.D, nk = (D + KT - 1) / KT;
+    const int D = a.D;
+    int flip = 0;
 
     for (int tile = tile0; tile < n_tiles; tile += a.tiles) {
         const Tile t = tile_of(a, s, tile);
@@ -187,60 +198,75 @@ __global__ __launch_bounds__(256) void attn_paged_rows_kernel(const Args a) {
 #pragma unroll
         for (int ks = 0; ks < NK; ++ks) {
             // a fragment that passes the end of the head is read from D - E on, as the keys' is; what an earlier one covers is zeroed
-            const int e0 = ks * KT + g * E, at = min(e0, D - E);
+            const int e0 = cb + ks * KT + g * E, at = min(e0, D - E);
             qf[ks] = __builtin_bit_cast(vec, load16(qrow + at));
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 if (at + e < e0 || !row_ok) qf[ks][e] = (T)0.f;
         }
-        f32x4 acc[NC][E];
+        f32x4 acc[E];
 #pragma unroll
-        for (int ch = 0; ch < NC; ++ch)
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[ch][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m = -INFINITY, l = 0.f;            // of the lane's row, the same in its four lanes
+        for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;            // of the lane's row, the same in its four lanes (and in all slices)
 
         for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
             const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n);
-            for (int xb = (int)x0 + wave * KB; xb < x1; xb += 4 * KB) {
-                const int xl = min(xb + (lane & 31), x1 - 1);
-                const unsigned row = cache_row(a, s, t.kb + xl * t.ks);
-                unsigned vrow[8];
-                const T* kp[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) kp[h] = kbase + cache_offset(a, __shfl(row, h * 16 + c));
-#pragma unroll
-                for (int i = 0; i < 8; ++i) vrow[i] = __shfl(row, (i >> 2) * 16 + g * 4 + (i & 3));
-                // narrow heads ask for all keys and values of the turn together; wide ones, which the registers do not hold at
-                // once, for a half of the keys, then the other, then the values 16 E channels at a time
-                u32x4 kf[WIDE ? 1 : 2][NK], vf[WIDE ? 1 : NC][8];
+            int xb = (int)x0 + kg * KB;
+            unsigned row = xb < x1 ? cache_row(a, s, t.kb + min(xb + (lane & 31), x1 - 1) * t.ks) : BAD;
+            for (int xt = (int)x0; xt < x1; xt += KG * KB, xb += KG * KB, flip ^= 1) {
+                const bool on = xb < x1;         // the wave's turn has keys
+                if (NC == 1 && !on) break;
                 f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-                auto load_k = [&](int h) {
+                unsigned vrow[8];
+                u32x4 kf[2][NK], vf[8];
+                bool gaps = false;
+                if (on) {
+                    const T* kp[2];
 #pragma unroll
-                    for (int ks = 0; ks < NK; ++ks)
-                        if (ks < nk) kf[WIDE ? 0 : h][ks] = load16(kp[h] + min(ks * KT + g * E, D - E));
-                };
-                auto load_v = [&](int ch) {
+                    for (int h = 0; h < 2; ++h) kp[h] = kbase + cache_offset(a, __shfl(row, h * 16 + c));
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) vf[WIDE ? 0 : ch][i] = load16(vbase + cache_offset(a, vrow[i]) + min(ch * CH + c * E, D - E));
-                };
-                auto score = [&](int h) {
+                    for (int i = 0; i < 8; ++i) vrow[i] = __shfl(row, (i >> 2) * 16 + g * 4 + (i & 3));
+                    gaps = __any(row == BAD);
+                    if (cb < D) {
 #pragma unroll
-                    for (int ks = 0; ks < NK; ++ks)
-                        if (ks < nk) sc[h] = El<T>::mfma(__builtin_bit_cast(vec, kf[WIDE ? 0 : h][ks]), qf[ks], sc[h]);
-                };
-                load_k(0);
-                if constexpr (WIDE) score(0);
-                load_k(1);
-                if constexpr (!WIDE) {
+                        for (int ks = 0; ks < NK; ++ks)
+                            if (cb + ks * KT < D) {
 #pragma unroll
-                    for (int ch = 0; ch < NC; ++ch) load_v(ch);
-                    score(0);
+                                for (int h = 0; h < 2; ++h) kf[h][ks] = load16(kp[h] + min(cb + ks * KT + g * E, D - E));
+                            }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) vf[i] = load16(vbase + cache_offset(a, vrow[i]) + min(cb + c * E, D - E));
+                    }
+                    // the next turn's rows are asked for meanwhile
+                    const int xn = xb + KG * KB;
+                    if (xn < x1) row = cache_row(a, s, t.kb + min(xn + (lane & 31), x1 - 1) * t.ks);
+                    if (cb < D) {
+#pragma unroll
+                        for (int ks = 0; ks < NK; ++ks)
+                            if (cb + ks * KT < D) {
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) sc[h] = El<T>::mfma(__builtin_bit_cast(vec, kf[h][ks]), qf[ks], sc[h]);
+                            }
+                    }
                 }
-                score(1);
+                if constexpr (NC > 1) {
+                    if (on) {
+                        *reinterpret_cast<f32x4*>(sh.s[flip][wave][lane]) = sc[0];
+                        *reinterpret_cast<f32x4*>(sh.s[flip][wave][lane] + 4) = sc[1];
+                    }
+                    __syncthreads();
+                    if (!on) continue;
+                    // all slices add in the same order: their statistics are the same bit for bit
+                    sc[0] = sc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int u = 0; u < NC; ++u) {
+                        sc[0] += *reinterpret_cast<const f32x4*>(sh.s[flip][kg * NC + u][lane]);
+                        sc[1] += *reinterpret_cast<const f32x4*>(sh.s[flip][kg * NC + u][lane] + 4);
+                    }
+                }
                 // scores of keys h * 16 + g * 4 + r, i.e. of slot i = h * 4 + r
                 const int p0 = t.kb + xb * t.ks, p1 = t.kb + (xb + KB - 1) * t.ks;
-                const bool masked = xb + KB > x1 || p0 < all_lo || p1 >= all_hi || t.rows - t.row0 < 16 || __any(row == BAD);
+                const bool masked = xb + KB > x1 || p0 < all_lo || p1 >= all_hi || t.rows - t.row0 < 16 || gaps;
                 unsigned see = 0xffu;
                 if (masked) {
                     see = 0u;
@@ -253,64 +279,61 @@ __global__ __launch_bounds__(256) void attn_paged_rows_kernel(const Args a) {
                 float p[8], mx = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    p[i] = (see >> i) & 1u ? sc[i >> 2][i & 3] * a.c : -INFINITY;
-                    mx = fmaxf(mx, p[i]);
+                    p[i] = (see >> i) & 1u ? sc[i >> 2][i & 3] : -INFINITY;
+                    mx = fmaxf(mx, (see >> i) & 1u ? p[i] * a.c : -INFINITY);
                 }
                 mx = jb_rows_reduce(mx, [](float u, float v) { return fmaxf(u, v); });
                 const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.f : m_new;
                 const float alpha = __builtin_amdgcn_exp2f(m - base);
                 float sum = 0.f;
+                // (fused: the rounding of the running maximum is common to all probabilities, a score's own product is not rounded)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { p[i] = __builtin_amdgcn_exp2f(p[i] - base); sum += p[i]; }
+                for (int i = 0; i < 8; ++i) {
+                    p[i] = (see >> i) & 1u ? __builtin_amdgcn_exp2f(fmaf(p[i], a.c, -base)) : 0.f;
+                    sum += p[i];
+                }
                 sum = jb_rows_reduce(sum, [](float u, float v) { return u + v; });
                 l = l * alpha + sum;
                 m = m_new;
                 if (__any(alpha != 1.0f)) {
 #pragma unroll
-                    for (int ch = 0; ch < NC; ++ch)
-#pragma unroll
-                        for (int e = 0; e < E; ++e) acc[ch][e] *= alpha;
+                    for (int e = 0; e < E; ++e) acc[e] *= alpha;
                 }
+                if (cb >= D) continue;
                 // A value that is no number may sit in a row that some queries do not see, and 0 * NaN would reach them.  Where a
                 // turn is masked at all its values are looked at: such elements leave the operands, and enter below one key at a
                 // time, for the queries that see it.
                 unsigned odd = 0u;
-                vec ph, pl;
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const unsigned x = vf[i][h] & El<T>::EXP2;
+                            if constexpr (E == 4) {
+                                if (x == El<T>::EXP2) { odd |= 1u << i; vf[i][h] = 0u; }
+                            } else {
+                                const bool b0 = (x & 0xffffu) == (El<T>::EXP2 & 0xffffu), b1 = x >> 16 == El<T>::EXP2 >> 16;
+                                if (b0 || b1) { odd |= 1u << i; vf[i][h] &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0xffffu : 0xffffffffu); }
+                            }
+                        }
+                }
                 if constexpr (E == 8) {
+                    vec ph, pl;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) { ph[i] = (T)p[i]; pl[i] = (T)(p[i] - (float)ph[i]); }
-                }
-#pragma unroll
-                for (int ch = 0; ch < NC; ++ch) {
-                    if (ch * CH >= D) break;
-                    if constexpr (WIDE) load_v(ch);
-                    u32x4 (&w)[8] = vf[WIDE ? 0 : ch];
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-#pragma unroll
-                            for (int h = 0; h < 4; ++h) {
-                                const unsigned x = w[i][h] & El<T>::EXP2;
-                                if constexpr (E == 4) {
-                                    if (x == El<T>::EXP2) { odd |= 1u << i; w[i][h] = 0u; }
-                                } else {
-                                    const bool b0 = (x & 0xffffu) == (El<T>::EXP2 & 0xffffu), b1 = x >> 16 == El<T>::EXP2 >> 16;
-                                    if (b0 || b1) { odd |= 1u << i; w[i][h] &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0xffffu : 0xffffffffu); }
-                                }
-                            }
-                    }
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        if constexpr (E == 8) {
-                            const vec vt = gather(w, e, T());
-                            acc[ch][e] = El<T>::mfma(vt, ph, acc[ch][e]);
-                            acc[ch][e] = El<T>::mfma(vt, pl, acc[ch][e]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                acc[ch][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, w[i])[e], p[i], acc[ch][e], 0, 0, 0);
-                        }
+                        const vec vt = gather(vf, e, T());
+                        acc[e] = El<T>::mfma(vt, ph, acc[e]);
+                        acc[e] = El<T>::mfma(vt, pl, acc[e]);
                     }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, vf[i])[e], p[i], acc[e], 0, 0, 0);
                 }
                 if (__any(odd != 0u)) {
                     for (int i = 0; i < 8; ++i) {
@@ -325,103 +348,120 @@ __global__ __launch_bounds__(256) void attn_paged_rows_kernel(const Args a) {
                             const bool take = __shfl(see, gg * 16 + c) >> i & 1u;
                             const T* vp = vbase + cache_offset(a, __shfl(ri, gg * 16));
 #pragma unroll
-                            for (int ch = 0; ch < NC; ++ch)
+                            for (int r = 0; r < 4; ++r) {
+                                const vec w = __builtin_bit_cast(vec, load16(vp + min(cb + (g * 4 + r) * E, D - E)));
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    const vec w = __builtin_bit_cast(vec, load16(vp + min(ch * CH + (g * 4 + r) * E, D - E)));
-#pragma unroll
-                                    for (int e = 0; e < E; ++e) {
-                                        const float x = (float)w[e];
-                                        if (take && !(fabsf(x) < INFINITY)) acc[ch][e][r] += pk * x;
-                                    }
+                                for (int e = 0; e < E; ++e) {
+                                    const float x = (float)w[e];
+                                    if (take && !(fabsf(x) < INFINITY)) acc[e][r] += pk * x;
                                 }
+                            }
                         }
                     }
                 }
             }
         }
 
-        // ---- join the four waves' states -----------------------------------------------------------
-        __syncthreads();                          // the exchange of the previous tile has been read
-        if (g == 0) { s_ml[wave][c][0] = m; s_ml[wave][c][1] = l; }
-        __syncthreads();
-        float M = -INFINITY, L = 0.f;
+        // ---- the rows' states: joined over the waves side by side on the keys, written where they belong --------------------------
+        float M = m, L = l, mine = 1.f;
+        if constexpr (KG > 1) {
+            __syncthreads();                      // the exchange of the previous tile has been read
+            if (g == 0 && cb == 0) { sh.ml[kg][c][0] = m; sh.ml[kg][c][1] = l; }
+            __syncthreads();
+            M = -INFINITY; L = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, s_ml[w][c][0]);
-        const float base = M == -INFINITY ? 0.f : M;
+            for (int w = 0; w < KG; ++w) M = fmaxf(M, sh.ml[w][c][0]);
+            const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) L += s_ml[w][c][1] * __builtin_amdgcn_exp2f(s_ml[w][c][0] - base);
-        const float mine = __builtin_amdgcn_exp2f(m - base);
-        const float inv = n_act > 1 ? 1.f : L != 0.f ? 1.f / L : 0.f;         // nothing seen: zeros
-        // what this thread writes: E channels from ch * CH + (tid % 16) * E of row tid / 16
-        const int wr = threadIdx.x >> 4, wc = threadIdx.x & 15;
-        const int wR = t.row0 + wr, wi = (int)jb_div(min(wR, t.rows - 1), a.group);
-        const int64_t wt = s.t0 + t.j0 + wi * t.js;
-        const int wh = kvh * a.G + (min(wR, t.rows - 1) - wi * a.G);
+            for (int w = 0; w < KG; ++w) L += sh.ml[w][c][1] * __builtin_amdgcn_exp2f(sh.ml[w][c][0] - base);
+            mine = __builtin_amdgcn_exp2f(m - base);
+        }
+        // a state of several is joined with the others' by its own maximum and sum; nothing seen: zeros
+        mine *= n_act > 1 ? 1.f : L != 0.f ? 1.f / L : 0.f;
         if (n_act > 1 && wave == 0 && g == 0 && row_ok) {
             float* o = a.ml + (((int64_t)(s.t0 + j) * a.n_head + head) * a.splits + split) * 2;
             o[0] = M; o[1] = L;
         }
-#pragma unroll
-        for (int ch = 0; ch < NC; ++ch) {
-            if (ch * CH >= D) break;
-            if (ch) __syncthreads();
-            // a lane holds channels of pieces g * 4 + r: piece m's tile e is channel min(ch * CH + m * E, D - E) + e
+        auto put = [&](int64_t tok, int h, int at, const float* v) {
+            if (n_act > 1) {
+                float* o = a.part + (((tok * a.n_head + h) * a.splits + split) * (int64_t)D + at);
+                *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+                if constexpr (E == 8) *reinterpret_cast<u32x4_any*>(o + 4) = __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]});
+            } else {
+                T* o = (T*)a.out + tok * a.o_row + (int64_t)h * a.o_head + at;
+                if constexpr (E == 8) store8<T>(o, v);
+                else *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+            }
+        };
+        // a lane holds pieces g * 4 + r of its row: piece m's channels are min(cb + m * E, D - E) + e
+        if constexpr (KG == 1) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-#pragma unroll
-                for (int e = 0; e < E; e += 4) {
-                    *reinterpret_cast<f32x4*>(&s_o[wave][c][(g * 4 + r) * E + e]) =
-                        f32x4{acc[ch][e][r], acc[ch][e + 1][r], acc[ch][e + 2][r], acc[ch][e + 3][r]} * (mine * inv);
-                }
-            }
-            __syncthreads();
-            const int d0 = ch * CH + wc * E, at = min(d0, D - E);
-            if (wR < t.rows && d0 < D) {
                 float v[8];
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = (s_o[0][wr][wc * E + e] + s_o[1][wr][wc * E + e]) + (s_o[2][wr][wc * E + e] + s_o[3][wr][wc * E + e]);
-                if (n_act > 1) {
-                    float* o = a.part + (((wt * a.n_head + wh) * a.splits + split) * (int64_t)D + at);
+                for (int e = 0; e < E; ++e) v[e] = acc[e][r] * mine;
+                const int d0 = cb + (g * 4 + r) * E;
+                if (row_ok && d0 < D) put(s.t0 + j, head, min(d0, D - E), v);
+            }
+        } else {
 #pragma unroll
-                    for (int e = 0; e < E; ++e) o[e] = v[e];
-                } else {
-                    T* o = (T*)a.out + wt * a.o_row + (int64_t)wh * a.o_head + at;
-                    if constexpr (E == 8) store8<T>(o, v);
-                    else *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < E; e += 4)
+                    *reinterpret_cast<f32x4*>(&sh.o[wave][c][(g * 4 + r) * E + e]) = f32x4{acc[e][r], acc[e + 1][r], acc[e + 2][r], acc[e + 3][r]} * mine;
+            __syncthreads();
+            const int wr = threadIdx.x >> 4, wc = threadIdx.x & 15, wR = min(t.row0 + wr, t.rows - 1), wi = (int)jb_div(wR, a.group);
+#pragma unroll
+            for (int u = 0; u < NC; ++u) {
+                const int d0 = u * CH + wc * E;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    v[e] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < KG; ++w) v[e] += sh.o[w * NC + u][wr][wc * E + e];
                 }
+                if (t.row0 + wr < t.rows && d0 < D) put(s.t0 + t.j0 + wi * t.js, kvh * a.G + (wR - wi * a.G), min(d0, D - E), v);
             }
         }
     }
 }
 
-// Joins the splits' states of rows that were split: one workgroup per (sequence, kv head, tile), 16 threads a row.
+// Joins the splits' states of rows that were split: a wave a row of a tile, four channels a lane, the splits' weights one a lane.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_paged_join_kernel(const Args a) {
+__global__ __launch_bounds__(64) void attn_paged_join_kernel(const Args a, int tile_rows) {
     int64_t b = blockIdx.x;
+    const int wr = (int)(b % tile_rows); b /= tile_rows;
     const int tile0 = (int)(b % a.tiles); b /= a.tiles;
-    const int kvh = (int)(b % a.n_kv), si = (int)(b / a.n_kv);
+    const int kvh = (int)(b % a.n_kv), si = (int)(b / a.n_kv), lane = threadIdx.x;
     const Seq s = seq_of(a, si);
-    const int n_tiles = tiles_of(a, s.nq), wr = threadIdx.x >> 4, wc = threadIdx.x & 15;
+    const int n_tiles = tiles_of(a, s.nq);
     for (int tile = tile0; tile < n_tiles; tile += a.tiles) {
         const Tile t = tile_of(a, s, tile);
-        const int R = t.row0 + wr, n_act = active_splits(a, t.n);
-        if (R >= t.rows || n_act < 2) continue;
-        const int i = (int)jb_div(R, a.group);
-        const int64_t tok = s.t0 + t.j0 + i * t.js;
-        const int h = kvh * a.G + (R - i * a.G);
-        const float* ml = a.ml + (tok * a.n_head + h) * a.splits * 2;
-        const float* part = a.part + (tok * a.n_head + h) * a.splits * (int64_t)a.D;
-        float M = -INFINITY, L = 0.f;
-        for (int u = 0; u < n_act; ++u) M = fmaxf(M, ml[2 * u]);
-        const float base = M == -INFINITY ? 0.f : M;
-        for (int u = 0; u < n_act; ++u) L += ml[2 * u + 1] * __builtin_amdgcn_exp2f(ml[2 * u] - base);
-        const float inv = L != 0.f ? 1.f / L : 0.f;
-        T* o = (T*)a.out + tok * a.o_row + (int64_t)h * a.o_head;
-        for (int d = wc; d < a.D; d += 16) {
-            float v = 0.f;
-            for (int u = 0; u < n_act; ++u) v += part[(int64_t)u * a.D + d] * __builtin_amdgcn_exp2f(ml[2 * u] - base);
-            o[d] = (T)(v * inv);
+        const int n_act = active_splits(a, t.n);
+        if (n_act < 2) continue;
+        for (int R = t.row0 + wr; R < min(t.row0 + 16, t.rows); R += tile_rows) {
+            const int i = (int)jb_div(R, a.group);
+            const int64_t tok = s.t0 + t.j0 + i * t.js;
+            const int h = kvh * a.G + (R - i * a.G);
+            const float* ml = a.ml + (tok * a.n_head + h) * a.splits * 2;
+            const float* part = a.part + (tok * a.n_head + h) * a.splits * (int64_t)a.D;
+            const float m = lane < n_act ? ml[2 * lane] : -INFINITY, l = lane < n_act ? ml[2 * lane + 1] : 0.f;      // at most 64 splits
+            const float M = jb_wave_max(m), base = M == -INFINITY ? 0.f : M, e = __builtin_amdgcn_exp2f(m - base), L = jb_wave_sum(l * e);
+            const float w = L != 0.f ? e / L : 0.f;
+            T* o = (T*)a.out + tok * a.o_row + (int64_t)h * a.o_head;
+            // (a last piece begins four channels before the end: d_head is 8 at least.  All lanes stay: each holds a split's weight)
+            for (int d0 = 0; d0 < a.D; d0 += 256) {
+                const int d = min(d0 + lane * 4, a.D - 4);
+                f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+                for (int u = 0; u < n_act; ++u)
+                    v += __builtin_bit_cast(f32x4, *reinterpret_cast<const u32x4_any*>(part + (int64_t)u * a.D + d)) * jb_readlane(w, u);
+                if (d0 + lane * 4 < a.D) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[d + k] = (T)v[k];
+                }
+            }
         }
     }
 }
@@ -477,7 +517,7 @@ int check_args(const jb_attn_paged_args* a, const char* who) {
 }
 
 template <typename T, int NC> void launch_rows(const Args& k, int64_t wgs, hipStream_t s) {
-    attn_paged_rows_kernel<T, NC><<<(unsigned)wgs, 256, 0, s>>>(k);
+    attn_paged_rows_kernel<T, NC><<<(unsigned)wgs, Shape<T, NC>::WAVES * 64, 0, s>>>(k);
 }
 
 }  // namespace
@@ -518,13 +558,16 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
         k.ml = k.part + (int64_t)a->n_tokens * a->n_head * w.splits * a->d_head;
     }
     hipStream_t s = (hipStream_t)stream;
+    const int64_t most_rows = (int64_t)a->max_q * k.G;
+    const int tile_rows = (int)(most_rows < 16 ? most_rows : 16);
+    JB_REQUIRE(w.splits == 1 || wgs * tile_rows <= 0x7fffffff, "grid too large");
 #define JB_ROWS(T, CH)                                                            \
     do {                                                                          \
         if (a->d_head <= 128) launch_rows<T, 128 / CH>(k, wgs * w.splits, s);     \
         else if (a->d_head <= 256) launch_rows<T, 256 / CH>(k, wgs * w.splits, s);\
         else launch_rows<T, 512 / CH>(k, wgs * w.splits, s);                      \
         JB_CHECK_LAUNCH();                                                        \
-        if (w.splits > 1) attn_paged_join_kernel<T><<<(unsigned)wgs, 256, 0, s>>>(k); \
+        if (w.splits > 1) attn_paged_join_kernel<T><<<(unsigned)(wgs * tile_rows), 64, 0, s>>>(k, tile_rows); \
     } while (0)
     if (a->dtype == JB_F16) JB_ROWS(f16, 128);
     else if (a->dtype == JB_BF16) JB_ROWS(bf16, 128);
