@@ -13,19 +13,19 @@ template <typename T> struct El;
 template <> struct El<f16> {
     typedef f16x8 vec;
     static constexpr int E = 8;
-    static constexpr unsigned EXP2 = 0x7c007c00u;
+    static constexpr unsigned ABS = 0x7fff7fffu, STEP = 0x04000400u;      // of two elements: without the sign; the exponent's lowest bit
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct El<bf16> {
     typedef bf16x8 vec;
     static constexpr int E = 8;
-    static constexpr unsigned EXP2 = 0x7f807f80u;
+    static constexpr unsigned ABS = 0x7fff7fffu, STEP = 0x00800080u;
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct El<float> {
     typedef f32x4 vec;
     static constexpr int E = 4;
-    static constexpr unsigned EXP2 = 0x7f800000u;
+    static constexpr unsigned ABS = 0x7fffffffu, STEP = 0x00800000u;
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return jb_mfma(a, b, c); }
 };
 
@@ -42,6 +42,8 @@ struct Args {
     int n_tokens, n_seq, n_head, n_kv, G, D;
     int func, bc, window;
     int tiles, splits; unsigned chunk;                    // grid: row tiles per (sequence, kv head), key splits, keys of a split's turn
+    unsigned groups; int by_die;                 // order of the workgroups (place_of)
+    int aligned;                                 // pages of a multiple of 16 rows, consecutive positions
     float c;                                     // scale * log2(e)
 };
 
@@ -87,6 +89,7 @@ __device__ __forceinline__ Tile tile_of(const Args& a, const Seq& s, int tile) {
         case JB_ATTN_TRANSPOSE_BLOCK: t.ks = a.bc; t.kb = pl % a.bc; t.n = pl / a.bc + 1; break;
         default: t.kb = a.window ? max(pf - a.window + 1, 0) : 0; t.n = pl + 1 - t.kb;
     }
+    if (a.aligned && t.n > 0) { t.n += t.kb & 15; t.kb &= ~15; }        // halves of turns begin at multiples of 16
     return t;
 }
 // The positions [lo, hi) that the query at position p sees (of those its tile walks).
@@ -99,6 +102,21 @@ __device__ __forceinline__ void sees(const Args& a, int p, int& lo, int& hi) {
 }
 __device__ __forceinline__ int active_splits(const Args& a, int n) {
     return a.splits == 1 ? 1 : min(a.splits, max((int)(((unsigned)n + a.chunk - 1u) / a.chunk), 1));
+}
+
+// Workgroup b's work.  Workgroups go round the eight dies by number, and each die has its own L2: b % 8 picks the group of work items
+// that share memory -- one token a sequence: a sequence's keys under all heads, whose rows lie side by side; chunks: a head's keys
+// under all tiles -- and a die takes a group's items one after the other.  Where that would leave dies idle, or give them sequences of
+// different lengths (chunks whose heads are no multiple of eight), the items go round instead.
+__device__ __forceinline__ bool place_of(const Args& a, unsigned b, int& tile, int& split, int& kvh, int& si) {
+    const unsigned inner = a.tiles == 1 ? a.n_kv : a.tiles;
+    unsigned group, item;
+    if (a.by_die) { const unsigned r = b >> 3; item = r % inner; group = (r / inner) * 8 + (b & 7); }
+    else { item = b % inner; group = b / inner; }
+    if (group >= a.groups) return false;
+    if (a.tiles == 1) { si = (int)(group % a.n_seq); split = (int)(group / a.n_seq); kvh = (int)item; tile = 0; }
+    else { kvh = (int)(group % a.n_kv); group /= a.n_kv; si = (int)(group % a.n_seq); split = (int)(group / a.n_seq); tile = (int)item; }
+    return true;
 }
 
 // (page << page_shift) | row in page of a position; BAD where the table names no page.
@@ -148,7 +166,14 @@ template <typename T> __device__ __forceinline__ void store8(T* o, const float* 
 // NC slices of 16 E channels cover d_head, each a wave's: heads of up to 128 halfs have four waves side by side on the keys, every
 // one with a running maximum and sum of its own, joined through LDS at the end; wider heads NC waves to a turn of 32 keys, which add
 // up their parts of the scores through LDS (one barrier a turn).  One wave for a whole head of 480 channels held 512 registers, four
-// waves a compute unit, each request waiting for the one before: 238 us for 16 sequences of 4096-8192 keys, now MEASURED.
+// waves a compute unit, each request waiting for the one before.
+// ALIGNED (pages of a multiple of 16 rows, keys at consecutive positions): a 16-key half of a turn lies in one page, so that its rows
+// are one scalar address and a lane's constant offset, page numbers come 64 at a time, and the next turn's rows are on their way while
+// one is computed.  Otherwise (odd pages, the transpose pattern) every key is looked up by a lane and its address handed round.
+// Measured (one new token a sequence; a copy reaches 4.8 TB/s on the card): 64 sequences of 511-8192 keys, 32 heads on 8 of 128 channels,
+// bf16 in pages of 16: 261 us, 4.4 TB/s; 16 of 4096-8192 under a head of 480, f16: 43 us, 4.4 TB/s; 64 of 500-4000, 8 heads of 150: 171 us, 4.1 TB/s.
+// Bound by memory.  Three waves a SIMD instead of two, for which the registers spill: 353, 61 and 259 us.  Keys looked up lane by lane
+// instead of ALIGNED: 345, 70 and 350 us.
 template <typename T, int NC> struct Shape {
     static constexpr int WAVES = NC > 4 ? NC : 4, KG = WAVES / NC, CH = 16 * El<T>::E, LDO = CH + 4;     // LDO: rows 4 banks apart
     struct Shared {
@@ -157,8 +182,8 @@ template <typename T, int NC> struct Shape {
         float ml[KG][16][2];
     };
 };
-template <typename T, int NC>
-__global__ __launch_bounds__((Shape<T, NC>::WAVES * 64)) void attn_paged_rows_kernel(const Args a) {
+template <typename T, int NC, bool ALIGNED>
+__global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows_kernel(const Args a) {
     typedef typename El<T>::vec vec;
     typedef Shape<T, NC> Sh;
     constexpr int E = El<T>::E, CH = Sh::CH, KT = 4 * E, NK = CH / KT, KG = Sh::KG;
@@ -166,16 +191,24 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64)) void attn_paged_rows_ke
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     // scalar, so that what depends on the wave branches: matrix instructions run whatever the lanes' mask, also under an empty one
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / NC, cb = wave % NC * CH;
-    int64_t b = blockIdx.x;
-    const int tile0 = (int)(b % a.tiles); b /= a.tiles;
-    const int split = (int)(b % a.splits); b /= a.splits;
-    const int kvh = (int)(b % a.n_kv), si = (int)(b / a.n_kv);
+    int tile0, split, kvh, si;
+    if (!place_of(a, blockIdx.x, tile0, split, kvh, si)) return;
     const Seq s = seq_of(a, si);
     const int n_tiles = tiles_of(a, s.nq);
     const T* kbase = (const T*)a.k + (int64_t)kvh * a.head_stride;
     const T* vbase = (const T*)a.v + (int64_t)kvh * a.head_stride;
-    const int D = a.D;
+    const int D = a.D, nk = min((D - cb + KT - 1) / KT, NK);       // k-tiles of this slice (none: a slice behind the head's end)
     int flip = 0;
+    // a lane's offsets from the row of its half's first key (ALIGNED): fragments' channels are clamped to the head
+    // -- bytes, so that an access is a scalar base and a 32-bit offset
+    const unsigned rs = (unsigned)a.row_stride * (unsigned)sizeof(T);
+    unsigned koff[NK], voff[4];
+    if constexpr (ALIGNED) {
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) koff[ks] = c * rs + (unsigned)min(cb + ks * KT + g * E, D - E) * (unsigned)sizeof(T);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) voff[r] = (g * 4 + r) * rs + (unsigned)min(cb + c * E, D - E) * (unsigned)sizeof(T);
+    }
 
     for (int tile = tile0; tile < n_tiles; tile += a.tiles) {
         const Tile t = tile_of(a, s, tile);
@@ -185,13 +218,19 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64)) void attn_paged_rows_ke
         const int R = t.row0 + c, my = min(R, t.rows - 1);
         const int qi = (int)jb_div(my, a.group), j = t.j0 + qi * t.js, head = kvh * a.G + (my - qi * a.G);
         const bool row_ok = R < t.rows;
-        int lo, hi;
-        sees(a, s.pos0 + j, lo, hi);
-        if (!row_ok) hi = lo;
-        // positions that every row of the tile sees: the first row ends first, the last begins last
-        int all_lo, all_hi, dummy;
-        sees(a, s.pos0 + t.j0 + (int)jb_div(t.row0, a.group) * t.js, dummy, all_hi);
-        sees(a, s.pos0 + t.j0 + (int)jb_div(min(t.row0 + 15, t.rows - 1), a.group) * t.js, all_lo, dummy);
+        // the walked keys [xlo, xhi) that the lane's row sees, and those that every row of the tile sees: the first row ends first, the
+        // last begins last.  (What rows that are none would add up stays in their own columns.)
+        auto walk = [&](int p, int& first, int& end) {
+            int lo, hi;
+            sees(a, p, lo, hi);
+            if (t.ks == 1) { first = max(lo - t.kb, 0); end = hi - t.kb; }
+            else { first = 0; end = p < 0 ? 0 : p / t.ks + 1; }
+        };
+        int xlo, xhi, all_lo, all_hi, unused;
+        walk(s.pos0 + j, xlo, xhi);
+        if (!row_ok || xhi < xlo) xlo = xhi = 0;
+        walk(s.pos0 + t.j0 + (int)jb_div(t.row0, a.group) * t.js, unused, all_hi);
+        walk(s.pos0 + t.j0 + (int)jb_div(min(t.row0 + 15, t.rows - 1), a.group) * t.js, all_lo, unused);
 
         const T* qrow = (const T*)a.q + (int64_t)(s.t0 + j) * a.q_row + (int64_t)head * a.q_head;
         vec qf[NK];
@@ -207,160 +246,230 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64)) void attn_paged_rows_ke
         f32x4 acc[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m = -INFINITY, l = 0.f;            // of the lane's row, the same in its four lanes (and in all slices)
+        float m = -INFINITY, l = 0.f;            // of the lane's row: the maximum the same in its four lanes, the sum a part in each
 
-        for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
-            const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n);
-            int xb = (int)x0 + kg * KB;
-            unsigned row = xb < x1 ? cache_row(a, s, t.kb + min(xb + (lane & 31), x1 - 1) * t.ks) : BAD;
-            for (int xt = (int)x0; xt < x1; xt += KG * KB, xb += KG * KB, flip ^= 1) {
-                const bool on = xb < x1;         // the wave's turn has keys
-                if (NC == 1 && !on) break;
-                f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-                unsigned vrow[8];
-                u32x4 kf[2][NK], vf[8];
-                bool gaps = false;
-                if (on) {
-                    const T* kp[2];
+        // One turn: the scores' parts so far in sc, the values in vf.  gone: bit i, no page holds key i.
+        auto turn = [&](f32x4 (&sc)[2], u32x4 (&vf)[8], int xb, int x1, unsigned gone, auto value_row) {
+            // scores of keys h * 16 + g * 4 + r, i.e. of slot i = h * 4 + r
+            const bool masked = xb + KB > x1 || xb < all_lo || xb + KB > all_hi || __any(gone != 0u);
+            unsigned see = 0xffu;
+            float p[8], mx = -INFINITY;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) kp[h] = kbase + cache_offset(a, __shfl(row, h * 16 + c));
+            for (int i = 0; i < 8; ++i) p[i] = sc[i >> 2][i & 3] * a.c;
+            if (masked) {
+                see = 0u;
+                const unsigned d0 = (unsigned)(xb + g * 4 - xlo), dn = (unsigned)(min(xhi, x1) > xlo ? min(xhi, x1) - xlo : 0);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) vrow[i] = __shfl(row, (i >> 2) * 16 + g * 4 + (i & 3));
-                    gaps = __any(row == BAD);
-                    if (cb < D) {
+                for (int i = 0; i < 8; ++i) see |= (d0 + (i >> 2) * 16 + (i & 3) < dn ? 1u : 0u) << i;
+                see &= ~gone;
 #pragma unroll
-                        for (int ks = 0; ks < NK; ++ks)
-                            if (cb + ks * KT < D) {
+                for (int i = 0; i < 8; ++i) p[i] = see >> i & 1u ? p[i] : -INFINITY;
+            }
 #pragma unroll
-                                for (int h = 0; h < 2; ++h) kf[h][ks] = load16(kp[h] + min(cb + ks * KT + g * E, D - E));
-                            }
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) vf[i] = load16(vbase + cache_offset(a, vrow[i]) + min(cb + c * E, D - E));
-                    }
-                    // the next turn's rows are asked for meanwhile
-                    const int xn = xb + KG * KB;
-                    if (xn < x1) row = cache_row(a, s, t.kb + min(xn + (lane & 31), x1 - 1) * t.ks);
-                    if (cb < D) {
-#pragma unroll
-                        for (int ks = 0; ks < NK; ++ks)
-                            if (cb + ks * KT < D) {
-#pragma unroll
-                                for (int h = 0; h < 2; ++h) sc[h] = El<T>::mfma(__builtin_bit_cast(vec, kf[h][ks]), qf[ks], sc[h]);
-                            }
-                    }
-                }
-                if constexpr (NC > 1) {
-                    if (on) {
-                        *reinterpret_cast<f32x4*>(sh.s[flip][wave][lane]) = sc[0];
-                        *reinterpret_cast<f32x4*>(sh.s[flip][wave][lane] + 4) = sc[1];
-                    }
-                    __syncthreads();
-                    if (!on) continue;
-                    // all slices add in the same order: their statistics are the same bit for bit
-                    sc[0] = sc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int u = 0; u < NC; ++u) {
-                        sc[0] += *reinterpret_cast<const f32x4*>(sh.s[flip][kg * NC + u][lane]);
-                        sc[1] += *reinterpret_cast<const f32x4*>(sh.s[flip][kg * NC + u][lane] + 4);
-                    }
-                }
-                // scores of keys h * 16 + g * 4 + r, i.e. of slot i = h * 4 + r
-                const int p0 = t.kb + xb * t.ks, p1 = t.kb + (xb + KB - 1) * t.ks;
-                const bool masked = xb + KB > x1 || p0 < all_lo || p1 >= all_hi || t.rows - t.row0 < 16 || gaps;
-                unsigned see = 0xffu;
-                if (masked) {
-                    see = 0u;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int x = xb + (i >> 2) * 16 + g * 4 + (i & 3), p = t.kb + x * t.ks;
-                        if (x < x1 && p >= lo && p < hi && vrow[i] != BAD) see |= 1u << i;
-                    }
-                }
-                float p[8], mx = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    p[i] = (see >> i) & 1u ? sc[i >> 2][i & 3] : -INFINITY;
-                    mx = fmaxf(mx, (see >> i) & 1u ? p[i] * a.c : -INFINITY);
-                }
-                mx = jb_rows_reduce(mx, [](float u, float v) { return fmaxf(u, v); });
-                const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.f : m_new;
+            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, p[i]);
+            mx = jb_rows_reduce(mx, [](float u, float v) { return fmaxf(u, v); });
+            const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.f : m_new;
+            if (__any(m_new != m)) {
                 const float alpha = __builtin_amdgcn_exp2f(m - base);
-                float sum = 0.f;
-                // (fused: the rounding of the running maximum is common to all probabilities, a score's own product is not rounded)
+                l *= alpha;
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] *= alpha;
+                m = m_new;
+            }
+            // (fused: the rounding of the running maximum is common to all probabilities, a score's own product is not rounded)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], a.c, -base));
+            // A value that is no number may sit in a row that some queries do not see, and 0 * NaN would reach them.  Where a
+            // turn is masked at all its values are looked at: such elements leave the operands, and enter below one key at a
+            // time, for the queries that see it.
+            unsigned odd = 0u;
+            if (masked) {
+                const unsigned left = (unsigned)max(x1 - xb - g * 4, 0);       // keys that are there at all: before the end, on a page
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    p[i] = (see >> i) & 1u ? __builtin_amdgcn_exp2f(fmaf(p[i], a.c, -base)) : 0.f;
-                    sum += p[i];
-                }
-                sum = jb_rows_reduce(sum, [](float u, float v) { return u + v; });
-                l = l * alpha + sum;
-                m = m_new;
-                if (__any(alpha != 1.0f)) {
+                    p[i] = see >> i & 1u ? p[i] : 0.f;
+                    const unsigned there = (unsigned)((i >> 2) * 16 + (i & 3)) < left && !(gone >> i & 1u) ? 0xffffffffu : 0u;
+                    unsigned any = 0u;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] *= alpha;
-                }
-                if (cb >= D) continue;
-                // A value that is no number may sit in a row that some queries do not see, and 0 * NaN would reach them.  Where a
-                // turn is masked at all its values are looked at: such elements leave the operands, and enter below one key at a
-                // time, for the queries that see it.
-                unsigned odd = 0u;
-                if (masked) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            const unsigned x = vf[i][h] & El<T>::EXP2;
-                            if constexpr (E == 4) {
-                                if (x == El<T>::EXP2) { odd |= 1u << i; vf[i][h] = 0u; }
-                            } else {
-                                const bool b0 = (x & 0xffffu) == (El<T>::EXP2 & 0xffffu), b1 = x >> 16 == El<T>::EXP2 >> 16;
-                                if (b0 || b1) { odd |= 1u << i; vf[i][h] &= (b0 ? 0xffff0000u : 0xffffffffu) & (b1 ? 0xffffu : 0xffffffffu); }
-                            }
-                        }
-                }
-                if constexpr (E == 8) {
-                    vec ph, pl;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) { ph[i] = (T)p[i]; pl[i] = (T)(p[i] - (float)ph[i]); }
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const vec vt = gather(vf, e, T());
-                        acc[e] = El<T>::mfma(vt, ph, acc[e]);
-                        acc[e] = El<T>::mfma(vt, pl, acc[e]);
+                    for (int h = 0; h < 4; ++h) {
+                        const unsigned w = vf[i][h] & there;
+                        // the top bit of an element: all of its exponent's are set (an addition carries into it)
+                        const unsigned bad = ((w & El<T>::ABS) + El<T>::STEP) & ~El<T>::ABS;
+                        vf[i][h] = w & ~(E == 8 ? (bad - (bad >> 15)) | bad : (unsigned)((int)bad >> 31));
+                        any |= bad;
                     }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-#pragma unroll
-                        for (int e = 0; e < E; ++e)
-                            acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, vf[i])[e], p[i], acc[e], 0, 0, 0);
+                    odd |= (any != 0u ? 1u : 0u) << i;
                 }
-                if (__any(odd != 0u)) {
-                    for (int i = 0; i < 8; ++i) {
-                        const unsigned long long who = __ballot(odd >> i & 1u);
-                        float pi = p[0];
-                        unsigned ri = vrow[0];
+            }
 #pragma unroll
-                        for (int u = 1; u < 8; ++u) { pi = u == i ? p[u] : pi; ri = u == i ? vrow[u] : ri; }
-                        for (int gg = 0; gg < 4; ++gg) {
-                            if ((who >> (16 * gg) & 0xffffull) == 0) continue;
-                            const float pk = __shfl(pi, gg * 16 + c);
-                            const bool take = __shfl(see, gg * 16 + c) >> i & 1u;
-                            const T* vp = vbase + cache_offset(a, __shfl(ri, gg * 16));
+            for (int i = 0; i < 8; ++i) l += p[i];
+            if (nk <= 0) return;
+            if constexpr (E == 8) {
+                vec ph, pl;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const vec w = __builtin_bit_cast(vec, load16(vp + min(cb + (g * 4 + r) * E, D - E)));
+                for (int i = 0; i < 8; ++i) { ph[i] = (T)p[i]; pl[i] = (T)(p[i] - (float)ph[i]); }
 #pragma unroll
-                                for (int e = 0; e < E; ++e) {
-                                    const float x = (float)w[e];
-                                    if (take && !(fabsf(x) < INFINITY)) acc[e][r] += pk * x;
-                                }
+                for (int e = 0; e < E; ++e) {
+                    const vec vt = gather(vf, e, T());
+                    acc[e] = El<T>::mfma(vt, ph, acc[e]);
+                    acc[e] = El<T>::mfma(vt, pl, acc[e]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, vf[i])[e], p[i], acc[e], 0, 0, 0);
+            }
+            if (__any(odd != 0u)) {
+                for (int i = 0; i < 8; ++i) {
+                    const unsigned long long who = __ballot(odd >> i & 1u);
+                    float pi = p[0];
+#pragma unroll
+                    for (int u = 1; u < 8; ++u) pi = u == i ? p[u] : pi;
+                    for (int gg = 0; gg < 4; ++gg) {
+                        if ((who >> (16 * gg) & 0xffffull) == 0) continue;
+                        const float pk = __shfl(pi, gg * 16 + c);
+                        const bool take = __shfl(see, gg * 16 + c) >> i & 1u;
+                        const T* vp = value_row(i, gg);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const vec w = __builtin_bit_cast(vec, load16(vp + min(cb + (g * 4 + r) * E, D - E)));
+#pragma unroll
+                            for (int e = 0; e < E; ++e) {
+                                const float x = (float)w[e];
+                                if (take && !(fabsf(x) < INFINITY)) acc[e][r] += pk * x;
                             }
                         }
                     }
                 }
             }
+        };
+        // the slices' parts of a turn's scores, added up in the same order by all: their statistics are the same bit for bit
+        auto add_slices = [&](f32x4 (&sc)[2], bool on) {
+            if (on) {
+                *reinterpret_cast<f32x4*>(sh.s[flip][wave][lane]) = sc[0];
+                *reinterpret_cast<f32x4*>(sh.s[flip][wave][lane] + 4) = sc[1];
+            }
+            __syncthreads();
+            if (on) {
+                sc[0] = sc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < NC; ++u) {
+                    sc[0] += *reinterpret_cast<const f32x4*>(sh.s[flip][kg * NC + u][lane]);
+                    sc[1] += *reinterpret_cast<const f32x4*>(sh.s[flip][kg * NC + u][lane] + 4);
+                }
+            }
+            flip ^= 1;
+        };
+
+        for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
+            const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n);
+            const int turns = (x1 - (int)x0 + KG * KB - 1) / (KG * KB);      // of every wave; the last may hold no keys for some
+            if constexpr (ALIGNED) {
+                u32x4 kf[2][NK], vf[8];
+                unsigned pages = 0;              // lane 2 u + h: the page of half h of the u-th turn of 32
+                // where half h of turn u begins (a half behind the last key: the last key's)
+                auto half_at = [&](int u, int h) { return t.kb + min((int)x0 + (u * KG + kg) * KB + h * 16, (x1 - 1) & ~15); };
+                int64_t row_at[2];               // the halves' first rows: of the turn whose keys, then whose values are asked for
+                unsigned gone = 0u;
+                auto find = [&](int u) {
+                    if ((u & 31) == 0) pages = (unsigned)s.table[jb_div((unsigned)half_at(u + (lane >> 1), lane & 1), a.page)];
+                    gone = 0u;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const unsigned pg = (unsigned)__builtin_amdgcn_readlane((int)pages, (u & 31) * 2 + h), at = (unsigned)half_at(u, h);
+                        if (pg >= a.n_pages) gone |= 0xfu << (4 * h);
+                        row_at[h] = (int64_t)(pg < a.n_pages ? pg : 0u) * a.page_stride + (int64_t)(at - jb_div(at, a.page) * a.page.d) * a.row_stride;
+                    }
+                };
+                auto load_k = [&]() {
+#pragma unroll
+                    for (int ks = 0; ks < NK; ++ks)
+                        if (NC == 1 || ks < nk) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) kf[h][ks] = load16((const char*)(kbase + row_at[h]) + koff[ks]);
+                        }
+                };
+                auto load_v = [&]() {
+                    if (NC == 1 || nk > 0) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) vf[i] = load16((const char*)(vbase + row_at[i >> 2]) + voff[i & 3]);
+                    }
+                };
+                find(0);
+                load_k();
+                load_v();
+                for (int u = 0; u < turns; ++u) {
+                    const int xb = (int)x0 + (u * KG + kg) * KB;
+                    const bool on = xb < x1;
+                    f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+                    if (on) {
+#pragma unroll
+                        for (int ks = 0; ks < NK; ++ks)
+                            if (NC == 1 || ks < nk) {
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) sc[h] = El<T>::mfma(__builtin_bit_cast(vec, kf[h][ks]), qf[ks], sc[h]);
+                            }
+                    }
+                    // the next turn's keys take the registers of this one's, and are on their way while it goes on; its values later
+                    // those of this one's
+                    const unsigned lost = gone;
+                    const int64_t at[2] = {row_at[0], row_at[1]};
+                    if (u + 1 < turns) { find(u + 1); load_k(); }
+                    if constexpr (NC > 1) add_slices(sc, on);
+                    if (on) turn(sc, vf, xb, x1, lost, [&](int i, int gg) { return vbase + at[i >> 2] + (int64_t)(gg * 4 + (i & 3)) * a.row_stride; });
+                    if (u + 1 < turns) load_v();
+                }
+            } else {
+                int xb = (int)x0 + kg * KB;
+                unsigned row = xb < x1 ? cache_row(a, s, t.kb + min(xb + (lane & 31), x1 - 1) * t.ks) : BAD;
+                for (int u = 0; u < turns; ++u, xb += KG * KB) {
+                    const bool on = xb < x1;     // the wave's turn has keys
+                    f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+                    unsigned vrow[8], gone = 0u;
+                    u32x4 vf[8];
+                    if (on) {
+                        u32x4 kf[2][NK];
+                        const T* kp[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) kp[h] = kbase + cache_offset(a, __shfl(row, h * 16 + c));
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            vrow[i] = __shfl(row, (i >> 2) * 16 + g * 4 + (i & 3));
+                            gone |= (vrow[i] == BAD ? 1u : 0u) << i;
+                        }
+#pragma unroll
+                        for (int ks = 0; ks < NK; ++ks)
+                            if (NC == 1 || ks < nk) {
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) kf[h][ks] = load16(kp[h] + min(cb + ks * KT + g * E, D - E));
+                            }
+                        if (NC == 1 || nk > 0) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) vf[i] = load16(vbase + cache_offset(a, vrow[i]) + min(cb + c * E, D - E));
+                        }
+                        // the next turn's rows are looked up meanwhile
+                        const int xn = xb + KG * KB;
+                        if (xn < x1) row = cache_row(a, s, t.kb + min(xn + (lane & 31), x1 - 1) * t.ks);
+#pragma unroll
+                        for (int ks = 0; ks < NK; ++ks)
+                            if (NC == 1 || ks < nk) {
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) sc[h] = El<T>::mfma(__builtin_bit_cast(vec, kf[h][ks]), qf[ks], sc[h]);
+                            }
+                    }
+                    if constexpr (NC > 1) add_slices(sc, on);
+                    if (on) turn(sc, vf, xb, x1, gone, [&](int i, int gg) {
+                        unsigned r = vrow[0];
+#pragma unroll
+                        for (int q = 1; q < 8; ++q) r = q == i ? vrow[q] : r;
+                        return vbase + cache_offset(a, __shfl(r, gg * 16));
+                    });
+                }
+            }
         }
+        l = jb_rows_reduce(l, [](float u, float v) { return u + v; });
 
         // ---- the rows' states: joined over the waves side by side on the keys, written where they belong --------------------------
         float M = m, L = l, mine = 1.f;
@@ -427,15 +536,16 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64)) void attn_paged_rows_ke
     }
 }
 
-// Joins the splits' states of rows that were split: a wave a row of a tile, four channels a lane, the splits' weights one a lane.
+// Joins the splits' states of rows that were split: a wave 64 channels of a row of a tile, four a lane, a quarter of the splits each
+// sixteen lanes; their weights one a lane.  (A wave a row left 16 waves to read 32 states of 480 channels: 19 us, now 5.)
 template <typename T>
 __global__ __launch_bounds__(64) void attn_paged_join_kernel(const Args a, int tile_rows) {
     int64_t b = blockIdx.x;
     const int wr = (int)(b % tile_rows); b /= tile_rows;
     const int tile0 = (int)(b % a.tiles); b /= a.tiles;
-    const int kvh = (int)(b % a.n_kv), si = (int)(b / a.n_kv), lane = threadIdx.x;
+    const int kvh = (int)(b % a.n_kv), si = (int)(b / a.n_kv), lane = threadIdx.x, part_of = lane >> 4;
     const Seq s = seq_of(a, si);
-    const int n_tiles = tiles_of(a, s.nq);
+    const int n_tiles = tiles_of(a, s.nq), d0 = blockIdx.y * 64 + (lane & 15) * 4, d = min(d0, a.D - 4);     // (a last piece begins four before the end)
     for (int tile = tile0; tile < n_tiles; tile += a.tiles) {
         const Tile t = tile_of(a, s, tile);
         const int n_act = active_splits(a, t.n);
@@ -445,22 +555,27 @@ __global__ __launch_bounds__(64) void attn_paged_join_kernel(const Args a, int t
             const int64_t tok = s.t0 + t.j0 + i * t.js;
             const int h = kvh * a.G + (R - i * a.G);
             const float* ml = a.ml + (tok * a.n_head + h) * a.splits * 2;
-            const float* part = a.part + (tok * a.n_head + h) * a.splits * (int64_t)a.D;
+            const float* part = a.part + (tok * a.n_head + h) * a.splits * (int64_t)a.D + d;
             const float m = lane < n_act ? ml[2 * lane] : -INFINITY, l = lane < n_act ? ml[2 * lane + 1] : 0.f;      // at most 64 splits
+            f32x4 v[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u)
+                if (u * 4 < n_act) v[u] = __builtin_bit_cast(f32x4, *reinterpret_cast<const u32x4_any*>(part + (int64_t)min(u * 4 + part_of, n_act - 1) * a.D));
             const float M = jb_wave_max(m), base = M == -INFINITY ? 0.f : M, e = __builtin_amdgcn_exp2f(m - base), L = jb_wave_sum(l * e);
             const float w = L != 0.f ? e / L : 0.f;
-            T* o = (T*)a.out + tok * a.o_row + (int64_t)h * a.o_head;
-            // (a last piece begins four channels before the end: d_head is 8 at least.  All lanes stay: each holds a split's weight)
-            for (int d0 = 0; d0 < a.D; d0 += 256) {
-                const int d = min(d0 + lane * 4, a.D - 4);
-                f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-                for (int u = 0; u < n_act; ++u)
-                    v += __builtin_bit_cast(f32x4, *reinterpret_cast<const u32x4_any*>(part + (int64_t)u * a.D + d)) * jb_readlane(w, u);
-                if (d0 + lane * 4 < a.D) {
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) o[d + k] = (T)v[k];
+            for (int u = 0; u < 16; ++u)
+                if (u * 4 < n_act) {
+                    const float wu = __shfl(w, u * 4 + part_of);          // (a lane behind the last split weighs nothing)
+                    o += v[u] * wu;
                 }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = jb_rows_reduce(o[k], [](float x, float y) { return x + y; });
+            if (part_of == 0 && d0 < a.D) {
+                T* q = (T*)a.out + tok * a.o_row + (int64_t)h * a.o_head + d;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q[k] = (T)o[k];
             }
         }
     }
@@ -474,16 +589,21 @@ Plan plan_of(const jb_attn_paged_args* p) {
     else w.tiles = (p->max_q * G + 15) / 16;
     // keys that a tile walks at most
     w.range = p->max_len;
-    if (p->attn_func == JB_ATTN_BLOCK || p->attn_func == JB_ATTN_PREV_BLOCK) w.range = bc + 16 / G;
+    if (p->attn_func == JB_ATTN_BLOCK || p->attn_func == JB_ATTN_PREV_BLOCK) w.range = bc + 16 / G + 15;
     else if (p->attn_func == JB_ATTN_TRANSPOSE_BLOCK) w.range = (p->max_len + bc - 1) / bc;
-    else if (p->window) w.range = (int64_t)p->window + 16 / G;
+    else if (p->window) w.range = (int64_t)p->window + 16 / G + 15;
     if (w.range > p->max_len) w.range = p->max_len;
     const int64_t wgs = w.tiles * p->n_kv_head * p->n_seq;
     w.splits = 1; w.chunk = 0x7fffffff;
-    if (wgs < 1024 && w.range > 256) {
-        int64_t chunk = (wgs * w.range / 2048 + 127) / 128 * 128;
-        if (chunk < 256) chunk = 256;
-        if ((w.range + chunk - 1) / chunk > 64) chunk = ((w.range + 63) / 64 + 127) / 128 * 128;
+    // Few tiles: the keys are split, so that every compute unit has two workgroups.  A workgroup costs some 5 us before its first keys
+    // are there, so its turn is 256 keys at least (16 sequences of 4096-8192 keys under one head of 480: 43 us; 512 keys: 55, 128: 58) -- a
+    // launch too small to fill the chip even so takes 64 (300 keys: 17 us against 32) -- and 2048 at most, which evens out
+    // sequences of different lengths (64 of 511-8192 keys: 261 us against 267 unsplit).
+    if (wgs < 1024 && w.range > 64) {
+        int64_t chunk = (wgs * w.range / 512 + 127) / 128 * 128;
+        if (chunk > 2048) chunk = 2048;
+        if (chunk < 256) chunk = wgs * w.range <= 64 * 256 ? 64 : 256;
+        if ((w.range + chunk - 1) / chunk > 64) chunk = ((w.range + 63) / 64 + 127) / 128 * 128;      // the join holds 64 states
         w.splits = (int)((w.range + chunk - 1) / chunk);
         w.chunk = (unsigned)chunk;
         if (w.splits < 2) { w.splits = 1; w.chunk = 0x7fffffff; }
@@ -517,7 +637,8 @@ int check_args(const jb_attn_paged_args* a, const char* who) {
 }
 
 template <typename T, int NC> void launch_rows(const Args& k, int64_t wgs, hipStream_t s) {
-    attn_paged_rows_kernel<T, NC><<<(unsigned)wgs, Shape<T, NC>::WAVES * 64, 0, s>>>(k);
+    if (k.aligned) attn_paged_rows_kernel<T, NC, true><<<(unsigned)wgs, Shape<T, NC>::WAVES * 64, 0, s>>>(k);
+    else attn_paged_rows_kernel<T, NC, false><<<(unsigned)wgs, Shape<T, NC>::WAVES * 64, 0, s>>>(k);
 }
 
 }  // namespace
@@ -553,6 +674,12 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     k.func = a->attn_func; k.bc = a->block_ctx > 0 ? a->block_ctx : 1; k.window = a->window;
     k.tiles = (int)w.tiles; k.splits = w.splits; k.chunk = w.chunk;
     k.c = a->scale * 1.44269504088896340736f;
+    // (a lane's offset inside a 16-row half is 32 bits wide)
+    k.aligned = a->page_size % 16 == 0 && a->attn_func != JB_ATTN_TRANSPOSE_BLOCK && a->row_stride <= 0x7fffffff / 64 - 512;
+    const int64_t inner = w.tiles == 1 ? k.n_kv : w.tiles, groups = wgs * w.splits / inner;
+    JB_REQUIRE((groups + 8) * inner <= 0x7fffffff, "grid too large");
+    k.groups = (unsigned)groups; k.by_die = w.tiles == 1 ? groups >= 8 : k.n_kv % 8 == 0;
+    const int64_t grid = k.by_die ? (groups + 7) / 8 * 8 * inner : groups * inner;
     if (need) {
         k.part = (float*)a->workspace;
         k.ml = k.part + (int64_t)a->n_tokens * a->n_head * w.splits * a->d_head;
@@ -563,11 +690,11 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     JB_REQUIRE(w.splits == 1 || wgs * tile_rows <= 0x7fffffff, "grid too large");
 #define JB_ROWS(T, CH)                                                            \
     do {                                                                          \
-        if (a->d_head <= 128) launch_rows<T, 128 / CH>(k, wgs * w.splits, s);     \
-        else if (a->d_head <= 256) launch_rows<T, 256 / CH>(k, wgs * w.splits, s);\
-        else launch_rows<T, 512 / CH>(k, wgs * w.splits, s);                      \
+        if (a->d_head <= 128) launch_rows<T, 128 / CH>(k, grid, s);               \
+        else if (a->d_head <= 256) launch_rows<T, 256 / CH>(k, grid, s);          \
+        else launch_rows<T, 512 / CH>(k, grid, s);                                \
         JB_CHECK_LAUNCH();                                                        \
-        if (w.splits > 1) attn_paged_join_kernel<T><<<(unsigned)(wgs * tile_rows), 64, 0, s>>>(k, tile_rows); \
+        if (w.splits > 1) attn_paged_join_kernel<T><<<dim3((unsigned)(wgs * tile_rows), (unsigned)((a->d_head + 63) / 64)), 64, 0, s>>>(k, tile_rows); \
     } while (0)
     if (a->dtype == JB_F16) JB_ROWS(f16, 128);
     else if (a->dtype == JB_BF16) JB_ROWS(bf16, 128);

@@ -5,6 +5,7 @@ in libjukebox_hip.so.  Tensors must live on the GPU and be contiguous; there is 
 """
 import ctypes as C
 import math
+from array import array
 
 import torch
 
@@ -307,43 +308,59 @@ def attn_prefill(func, q, kcache, vcache, n_head, block_ctx, t0):
 _PAGED_TYPES = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
 
 
-def _paged_type(*ts):
+def _paged_type(t, *ts):
     """dtype code of the paged cache's operators (single, half and bfloat16) for tensors that must share it."""
-    code = _PAGED_TYPES.get(ts[0].dtype)
-    if code is None or any(t.dtype != ts[0].dtype for t in ts):
-        raise L.JukeboxHipError(f"expected one type of float32, float16, bfloat16; got {', '.join(str(t.dtype) for t in ts)}")
+    dtype = t.dtype
+    code = _PAGED_TYPES.get(dtype)
+    for x in ts:
+        if x.dtype != dtype:
+            code = None
+    if code is None:
+        raise L.JukeboxHipError(f"expected one type of float32, float16, bfloat16; got {', '.join(str(x.dtype) for x in (t, *ts))}")
     return code
 
 
 def _chk_paged(first, *ts):
     """Every tensor on the first one's GPU."""
-    if not first.is_cuda or any(t is not None and t.device != first.device for t in ts):
-        raise L.JukeboxHipError("expected tensors on one GPU")
+    if not first.is_cuda:
+        raise L.JukeboxHipError("expected GPU tensors")
+    i = first.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != i:
+            raise L.JukeboxHipError("expected tensors on one GPU")
 
 
-def _chk_int(name, t, *shape):
-    """A contiguous int32 array; None in `shape`: any length."""
-    if t.dtype != torch.int32 or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)) or not t.is_contiguous():
-        raise L.JukeboxHipError(f"{name}: expected a contiguous int32 array of shape {tuple('*' if n is None else n for n in shape)}")
+def _chk_int(name, t, n=None):
+    """A contiguous int32 array (of n elements)."""
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+        raise L.JukeboxHipError(f"{name}: expected a contiguous int32 array" + ("" if n is None else f" of {n} elements"))
 
 
 def _chk_table(table):
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] == 0 or (table.shape[1] > 1 and table.stride(1) != 1):
+    if table.dtype != torch.int32 or table.dim() != 2:
         raise L.JukeboxHipError("table: expected int32 rows of page numbers")
-    # rows of a table of one row may carry any stride
-    stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
-    if stride < table.shape[1]:
+    n, width = table.shape
+    stride, one = table.stride()
+    if width == 0 or (width > 1 and one != 1):
+        raise L.JukeboxHipError("table: expected int32 rows of page numbers")
+    if n < 2:           # the row of a table of one row may carry any stride
+        stride = width
+    elif stride < width:
         raise L.JukeboxHipError("table: rows overlap")
-    return stride
+    return n, width, stride
 
 
-def _launch(fn, device, *args):
-    """A call of the library on the current stream of the tensors' own GPU."""
-    if device.index == torch.cuda.current_device():
-        L.check(fn(*args, L.stream()))
+def _launch(fn, t, *args):
+    """A call of the library on the current stream of tensor t's own GPU."""
+    i = t.get_device()
+    # (the raw handles: a Stream object and its device index cost more than the rest of a small call)
+    if i == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
-        with torch.cuda.device(device):
-            L.check(fn(*args, L.stream()))
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        L.check(rc)
 
 
 def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, func=0, block_ctx=0, window=0, scale=None, out=None):
@@ -361,8 +378,7 @@ def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, fun
         raise L.JukeboxHipError("expected q (n_tokens, n_head, d_head) and kpool, vpool (n_pages, page_size, n_kv_head, d_head) of equal strides")
     T, H, D = q.shape
     P, page, KV, _ = kpool.shape
-    table_stride = _chk_table(table)
-    n = table.shape[0]
+    n, width, table_stride = _chk_table(table)
     _chk_int("lens", lens, n)
     _chk_int("cu_q", cu_q, n + 1)
     if out is None:
@@ -374,16 +390,17 @@ def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, fun
     ps, rs, hs = kpool.stride()[:3]
     a = L.AttnPagedArgs(code, func, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0) if T > 1 else H * D,
                         out.stride(1) if H > 1 else D, kpool.data_ptr(), vpool.data_ptr(), ps, rs, hs, P, page, table.data_ptr(),
-                        table_stride, table.shape[1], lens.data_ptr(), cu_q.data_ptr(), T, n, H, KV, D, T if max_q is None else min(max_q, T),
-                        min(table.shape[1] * page if max_len is None else max_len, 0x7fffffff), block_ctx or 0, window or 0,
+                        table_stride, width, lens.data_ptr(), cu_q.data_ptr(), T, n, H, KV, D, T if max_q is None else min(max_q, T),
+                        min(width * page if max_len is None else max_len, 0x7fffffff), block_ctx or 0, window or 0,
                         1.0 / math.sqrt(D) if scale is None else scale, None, 0)
-    need = L.lib().jb_attn_paged_workspace(C.byref(a))
+    lib = L.lib()
+    need = lib.jb_attn_paged_workspace(C.byref(a))
     if need < 0:
         L.check(need)
     if need:            # the caching allocator keeps it for this stream (or this captured graph) until the launches have run
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    _launch(L.lib().jb_attn_paged, q.device, C.byref(a))
+    _launch(lib.jb_attn_paged, q, C.byref(a))
     return out
 
 
@@ -406,19 +423,18 @@ def kv_write(k, v, kpool, vpool, slots):
         hs = phs = D
     a = L.KvWriteArgs(code, k.data_ptr(), v.data_ptr(), ts, hs, kpool.data_ptr(), vpool.data_ptr(), ps, rs, phs, kpool.shape[0],
                       kpool.shape[1], slots.data_ptr(), T, KV, D)
-    _launch(L.lib().jb_kv_write, k.device, C.byref(a))
+    _launch(L.lib().jb_kv_write, k, C.byref(a))
 
 
 def _page_table(table, lens, ref, page_size, status=None):
-    stride = _chk_table(table)
-    n = table.shape[0]
+    n, width, stride = _chk_table(table)
     if lens is not None:
         _chk_int("lens", lens, n)
-    _chk_int("ref", ref, None)
+    _chk_int("ref", ref)
     if status is not None:
         _chk_int("status", status, 1)
     _chk_paged(table, lens, ref, status)
-    return L.PageTable(table.data_ptr(), stride, n, table.shape[1], L.ptr(lens), ref.data_ptr(), ref.shape[0], page_size)
+    return L.PageTable(table.data_ptr(), stride, n, width, L.ptr(lens), ref.data_ptr(), ref.shape[0], page_size)
 
 
 def _page_pools(pools, n_pages, device):
@@ -426,7 +442,7 @@ def _page_pools(pools, n_pages, device):
     if len(pools) == 0:
         return L.PagePools(None, 0, n_pages, 1, 1)
     p = pools[0]
-    shape, stride, size = p.shape, p.stride(), p.element_size()
+    shape, stride, dtype, size, gpu = p.shape, p.stride(), p.dtype, p.element_size(), device.index
     n = 1
     for m, st in zip(reversed(shape[1:]), reversed(stride[1:])):
         if m > 1 and st != n:
@@ -435,10 +451,10 @@ def _page_pools(pools, n_pages, device):
     if shape[0] != n_pages or n == 0 or (n_pages > 1 and stride[0] < n):
         raise L.JukeboxHipError(f"pools: expected {n_pages} pages that do not overlap")
     for x in pools:
-        if x.shape != shape or x.stride() != stride or x.element_size() != size or x.device != device:
+        if x.shape != shape or x.stride() != stride or x.dtype != dtype or x.get_device() != gpu:
             raise L.JukeboxHipError("pools: expected equal shapes, strides and types on the table's GPU")
-    base = (L.vp * len(pools))(*[x.data_ptr() for x in pools])
-    return L.PagePools(base, len(pools), n_pages, n * size, (stride[0] if n_pages > 1 else n) * size)
+    base = (C.c_uint64 * len(pools)).from_buffer(array("Q", [x.data_ptr() for x in pools]))
+    return L.PagePools(C.cast(base, C.POINTER(L.vp)), len(pools), n_pages, n * size, (stride[0] if n_pages > 1 else n) * size)
 
 
 def pages_extend(table, lens, ref, cu_new, page_size, n_tokens, status):
@@ -450,16 +466,16 @@ def pages_extend(table, lens, ref, cu_new, page_size, n_tokens, status):
     _chk_paged(table, cu_new)
     slots = torch.empty(n_tokens, dtype=torch.int64, device=table.device)
     work = torch.empty(1 + 2 * t.n_seq + t.n_pages, dtype=torch.int32, device=table.device)
-    _launch(L.lib().jb_pages_extend, table.device, C.byref(t), cu_new.data_ptr(), n_tokens, slots.data_ptr(), work.data_ptr(), status.data_ptr())
+    _launch(L.lib().jb_pages_extend, table, C.byref(t), cu_new.data_ptr(), n_tokens, slots.data_ptr(), work.data_ptr(), status.data_ptr())
     return slots
 
 
 def pages_free(table, lens, ref, rows, status):
     """The sequences in these rows (int32) of the table end (jb_pages_free): references given back, rows -1, lengths 0."""
     t = _page_table(table, lens, ref, 1, status)
-    _chk_int("rows", rows, None)
+    _chk_int("rows", rows)
     _chk_paged(table, rows)
-    _launch(L.lib().jb_pages_free, table.device, C.byref(t), rows.data_ptr(), rows.shape[0], status.data_ptr())
+    _launch(L.lib().jb_pages_free, table, C.byref(t), rows.data_ptr(), rows.shape[0], status.data_ptr())
 
 
 def pages_fork(pools, table, lens, ref, src, dst, page_size, status):
@@ -468,11 +484,11 @@ def pages_fork(pools, table, lens, ref, src, dst, page_size, status):
     pages.  The rows dst are empty before (pages_free), and no source."""
     t = _page_table(table, lens, ref, page_size, status)
     p = _page_pools(pools, t.n_pages, table.device)
-    _chk_int("src", src, None)
+    _chk_int("src", src)
     _chk_int("dst", dst, src.shape[0])
     _chk_paged(table, src, dst)
     work = torch.empty(2 + 4 * src.shape[0], dtype=torch.int32, device=table.device)
-    _launch(L.lib().jb_pages_fork, table.device, C.byref(t), C.byref(p), src.data_ptr(), dst.data_ptr(), src.shape[0], work.data_ptr(), status.data_ptr())
+    _launch(L.lib().jb_pages_fork, table, C.byref(t), C.byref(p), src.data_ptr(), dst.data_ptr(), src.shape[0], work.data_ptr(), status.data_ptr())
 
 
 def pages_compact(pools, table, ref):
@@ -482,7 +498,7 @@ def pages_compact(pools, table, ref):
     p = _page_pools(pools, t.n_pages, table.device)
     table_out, ref_out = torch.empty(table.shape, dtype=torch.int32, device=table.device), torch.empty_like(ref)
     work = torch.empty(2 + 3 * t.n_pages, dtype=torch.int32, device=table.device)
-    _launch(L.lib().jb_pages_compact, table.device, C.byref(t), C.byref(p), table_out.data_ptr(), ref_out.data_ptr(), work.data_ptr())
+    _launch(L.lib().jb_pages_compact, table, C.byref(t), C.byref(p), table_out.data_ptr(), ref_out.data_ptr(), work.data_ptr())
     return table_out, ref_out
 
 
@@ -491,10 +507,10 @@ def pages_copy(pools, src, dst):
     if len(pools) == 0:
         return
     p = _page_pools(pools, pools[0].shape[0], pools[0].device)
-    _chk_int("src", src, None)
+    _chk_int("src", src)
     _chk_int("dst", dst, src.shape[0])
     _chk_paged(pools[0], src, dst)
-    _launch(L.lib().jb_pages_copy, src.device, C.byref(p), src.data_ptr(), dst.data_ptr(), src.shape[0])
+    _launch(L.lib().jb_pages_copy, src, C.byref(p), src.data_ptr(), dst.data_ptr(), src.shape[0])
 
 
 def vq_gather(codes, codebook):
@@ -558,5 +574,5 @@ def sample_filtered(logits, u, temp=1.0, top_k=0, top_p=0.0, min_p=0.0, out=None
             vals.append(x)
     _chk_paged(logits, out, *each)
     a = L.SampleFilteredArgs(code, logits.data_ptr(), logits.stride(0) if n > 1 else bins, n, bins, *ptrs, *vals[1:], out.data_ptr())
-    _launch(L.lib().jb_sample_filtered, logits.device, C.byref(a))
+    _launch(L.lib().jb_sample_filtered, logits, C.byref(a))
     return out
