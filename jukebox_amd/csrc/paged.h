@@ -4,6 +4,7 @@
 
 typedef __bf16 bf16;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 // 16 bytes at any address that the element type allows (a head of 150 halfs starts at an odd multiple of 4 bytes): global memory
 // takes a dword-x4 access at such an address as one instruction

@@ -41,10 +41,11 @@ struct Args {
     int page_shift;                              // ceil(log2 page_size): a row of the cache is (page << page_shift) | row in page
     int n_tokens, n_seq, n_head, n_kv, G, D;
     int func, bc, window;
+    int tr;                                      // rows of a tile
     int tiles, splits; unsigned chunk;                    // grid: row tiles per (sequence, kv head), key splits, keys of a split's turn
     unsigned groups; int by_die;                 // order of the workgroups (place_of)
     int aligned;                                 // pages of a multiple of 16 rows, consecutive positions
-    float c;                                     // scale * log2(e)
+    float c, c_abs;                              // scale * log2(e); its magnitude, not quite 0 (-inf * 0 is no number)
 };
 
 constexpr unsigned BAD = 0xffffffffu;            // a key on a page number that does not exist: nobody sees it
@@ -62,9 +63,9 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int i) {
     return s;
 }
 __device__ __forceinline__ int tiles_of(const Args& a, int nq) {
-    if (a.func != JB_ATTN_TRANSPOSE_BLOCK) return (int)(((int64_t)nq * a.G + 15) / 16);
+    if (a.func != JB_ATTN_TRANSPOSE_BLOCK) return (int)(((int64_t)nq * a.G + a.tr - 1) / a.tr);
     const int cls = min(a.bc, nq);
-    return cls == 0 ? 0 : cls * (int)(((int64_t)((nq + a.bc - 1) / a.bc) * a.G + 15) / 16);
+    return cls == 0 ? 0 : cls * (int)(((int64_t)((nq + a.bc - 1) / a.bc) * a.G + a.tr - 1) / a.tr);
 }
 // Row r of a tile is token j0 + i * js of the chunk, i = (row0 + r) / G, head (row0 + r) % G; the keys that any of its rows
 // may see sit at positions kb + x * ks, x < n.
@@ -72,16 +73,16 @@ struct Tile { int j0, js, row0, rows, kb, ks, n; };      // rows: rows of this t
 __device__ __forceinline__ Tile tile_of(const Args& a, const Seq& s, int tile) {
     Tile t;
     if (a.func == JB_ATTN_TRANSPOSE_BLOCK) {             // one residue class of positions modulo bc
-        const int per = (int)(((int64_t)((s.nq + a.bc - 1) / a.bc) * a.G + 15) / 16);
-        t.j0 = tile / per; t.js = a.bc; t.row0 = (tile % per) * 16;
+        const int per = (int)(((int64_t)((s.nq + a.bc - 1) / a.bc) * a.G + a.tr - 1) / a.tr);
+        t.j0 = tile / per; t.js = a.bc; t.row0 = (tile % per) * a.tr;
         t.rows = (s.nq - t.j0 + a.bc - 1) / a.bc * a.G;
     } else {
-        t.j0 = 0; t.js = 1; t.row0 = tile * 16; t.rows = s.nq * a.G;
+        t.j0 = 0; t.js = 1; t.row0 = tile * a.tr; t.rows = s.nq * a.G;
     }
     t.kb = 0; t.ks = 1; t.n = 0;
     if (t.row0 >= t.rows) return t;
     const int pf = max(s.pos0 + t.j0 + (int)jb_div(t.row0, a.group) * t.js, 0);
-    const int pl = s.pos0 + t.j0 + (int)jb_div(min(t.row0 + 15, t.rows - 1), a.group) * t.js;
+    const int pl = s.pos0 + t.j0 + (int)jb_div(min(t.row0 + a.tr, t.rows) - 1, a.group) * t.js;
     if (pl < 0) return t;                                // a length shorter than the chunk: no such positions
     switch (a.func) {
         case JB_ATTN_BLOCK: t.kb = pf - pf % a.bc; t.n = pl + 1 - t.kb; break;
@@ -115,7 +116,7 @@ __device__ __forceinline__ bool place_of(const Args& a, unsigned b, int& tile, i
     else { item = b % inner; group = b / inner; }
     if (group >= a.groups) return false;
     if (a.tiles == 1) { si = (int)(group % a.n_seq); split = (int)(group / a.n_seq); kvh = (int)item; tile = 0; }
-    else { kvh = (int)(group % a.n_kv); group /= a.n_kv; si = (int)(group % a.n_seq); split = (int)(group / a.n_seq); tile = (int)item; }
+    else { kvh = (int)(group % a.n_kv); group /= a.n_kv; si = (int)(group % a.n_seq); split = (int)(group / a.n_seq); tile = a.tiles - 1 - (int)item; }      // the longest first
     return true;
 }
 
@@ -536,6 +537,308 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
     }
 }
 
+// Chunks: one workgroup of four waves per (sequence, kv head, tile of 128 rows, split of the keys), a wave 32 rows.
+//
+// The same two products on 32 x 32 x 16 matrix instructions: S^T = K Q^T leaves a lane the scores of 16 of 32 keys for row l & 31, which
+// are the B operand of O^T += V^T P^T once slot (h, i) of a k-step s is key 16 s + 8 (i / 4) + 4 h + i % 4.  64 keys at a time go through LDS,
+// two buffers, one barrier a turn: half the waves bring the keys' rows, the others the values', transposed on the way by byte
+// permutations ([channel][key], so that an operand is one 16-byte read), all asked for a turn ahead.  LDS rows are padded by 16 bytes: the
+// 16 lanes of a read phase then hit 16 different groups of four banks.
+// The probabilities enter the second product rounded once to 16 bits, which adds an error of the size of the output's own
+// rounding (each is off by half a step, and they average); a second product for the rest would cost a quarter of the rate.
+// Measured (32 heads on 8 of 128 channels, bf16, pages of 64; the library's product of 16384^3 runs at 1370 TFLOP/s): 4 x 2048 queries behind
+// 6144 keys: 1.22 ms, 790 TFLOP/s; 4 x 257-2048 behind 4097-8192: 745 us, 635 TFLOP/s.  Two workgroups share a compute unit, and the
+// products' 27 % of the time hide behind the softmax's exponentials and the LDS reads, of which either alone would take about as long
+// as the products at their peak.  Waves of 64 rows, which halve the LDS reads but leave one wave a SIMD (and its registers spilling): 1.13 ms
+// instead of 0.83 for the second case as things then were.
+template <typename T> struct Mfma32;
+template <> struct Mfma32<f16> { static __device__ __forceinline__ f32x16 go(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); } };
+template <> struct Mfma32<bf16> { static __device__ __forceinline__ f32x16 go(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); } };
+
+template <int DP> struct ChunkLds {                                       // bytes
+    static constexpr int KROW = DP * 2 + 16, VROW = 64 * 2 + 16, K = 64 * KROW, V = DP * VROW, BUF = K + V;
+    static constexpr int OFF = 2 * BUF, ODD = OFF + 3 * 64 * 8, GAP = ODD + 4, ALL = GAP + 3 * 4;
+};
+__device__ __forceinline__ float swap_halves_max(float x) {              // the larger of lanes l and l ^ 32, in both
+    float a = x, b = x;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    return fmaxf(a, b);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_paged_chunk_kernel(const Args a) {
+    typedef typename El<T>::vec vec;
+    typedef ChunkLds<DP> L;
+    constexpr int NKS = DP / 16, NDT = DP / 32, PIECES = DP / 8, LPR = PIECES < 16 ? PIECES : 16, SETS = (PIECES + 15) / 16;
+    constexpr int CREW = PIECES > 8 ? 2 : 1;      // waves that bring the keys' rows, and as many the values': eight pieces a lane and set
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    // of the turn computed, the one asked for and the one looked up:
+    int64_t* const s_off = reinterpret_cast<int64_t*>(lds + L::OFF);    // [3][64]: a key's offset in the pool, -1: nowhere
+    int* const s_gap = reinterpret_cast<int*>(lds + L::GAP);            // [3]: whether a key is on no page
+    int* const s_odd = reinterpret_cast<int*>(lds + L::ODD);            // whether values have been met that are no numbers
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int tile0, split, kvh, si;
+    if (!place_of(a, blockIdx.x, tile0, split, kvh, si)) return;
+    const Seq s = seq_of(a, si);
+    const int n_tiles = tiles_of(a, s.nq), D = a.D, NP = (D + 7) / 8;
+    const T* kbase = (const T*)a.k + (int64_t)kvh * a.head_stride;
+    const T* vbase = (const T*)a.v + (int64_t)kvh * a.head_stride;
+    // pieces behind the head's end are zeros throughout (the queries' are too, but 0 * NaN is not)
+    if (NP < PIECES)
+        for (int i = threadIdx.x; i < 2 * 64 * (PIECES - NP); i += 256) {
+            const int row = i / (PIECES - NP), pc = NP + i % (PIECES - NP);
+            *reinterpret_cast<u32x4*>(lds + (row >> 6) * L::BUF + (row & 63) * L::KROW + pc * 16) = u32x4{0, 0, 0, 0};
+        }
+
+    for (int tile = tile0; tile < n_tiles; tile += a.tiles) {
+        const Tile t = tile_of(a, s, tile);
+        if (t.row0 >= t.rows) continue;
+        const int n_act = active_splits(a, t.n);
+        if (split >= n_act) continue;
+        auto pos_of = [&](int R) { return s.pos0 + (int)jb_div(R, a.group); };
+        auto walk = [&](int p, int& first, int& end) {
+            int lo, hi;
+            sees(a, p, lo, hi);
+            first = max(lo - t.kb, 0); end = max(hi - t.kb, 0);
+        };
+        vec qf[NKS];
+        const int R0 = t.row0 + wave * 32, R = R0 + c, my = min(R, t.rows - 1);
+        const int qi = (int)jb_div(my, a.group), head = kvh * a.G + my - qi * a.G;
+        const T* qrow = (const T*)a.q + (int64_t)(s.t0 + qi) * a.q_row + (int64_t)head * a.q_head;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+            const int e0 = (ks * 2 + h) * 8, at = min(e0, D - 8);
+            vec x = __builtin_bit_cast(vec, load16(qrow + at));
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (at + e < e0 || R >= t.rows) x[e] = (T)0.f;
+            if (a.c < 0.f) x = -x;                // (the softmax below takes a scale that is not negative)
+            qf[ks] = x;
+        }
+        // the walked keys that the lane's row sees; those that all of the wave's rows see, and any of them (a wave without rows: none)
+        int xlo, xhi, all_lo = 0x7fffffff, all_hi = 0, any_lo = 0x7fffffff, any_hi = 0;
+        walk(s.pos0 + qi, xlo, xhi);
+        if (R >= t.rows || xhi < xlo) xlo = xhi = 0;
+        if (R0 < t.rows) {
+            walk(pos_of(R0), any_lo, all_hi);
+            walk(pos_of(min(R0 + 31, t.rows - 1)), all_lo, any_hi);
+        }
+        // what every row of the workgroup sees: outside it the values are looked at on their way to LDS
+        int wg_lo, wg_hi, unused;
+        walk(pos_of(t.row0), unused, wg_hi);
+        walk(pos_of(min(t.row0 + a.tr, t.rows) - 1), wg_lo, unused);
+
+        f32x16 acc[NDT];
+        float m = -INFINITY, l = 0.f;            // of the lane's row: the maximum the same in both its lanes, the sum a part in each
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
+
+        __syncthreads();
+        if (threadIdx.x == 0) *s_odd = 0;
+        for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
+            const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n), turns = (x1 - (int)x0 + 63) / 64;
+            // the first wave: where the keys of turn u are -- their pages asked for early in a turn, used at its end
+            auto page_number = [&](int u) { return (unsigned)s.table[jb_div((unsigned)(t.kb + min((int)x0 + u * 64 + lane, x1 - 1)), a.page)]; };
+            auto look_up = [&](int u, unsigned pg) {
+                const int x = (int)x0 + u * 64 + lane;
+                const unsigned at = (unsigned)(t.kb + min(x, x1 - 1)), in_page = at - jb_div(at, a.page) * a.page.d;
+                s_off[u % 3 * 64 + lane] = x < x1 && pg < a.n_pages ? (int64_t)pg * a.page_stride + (int64_t)in_page * a.row_stride : -1;
+                const bool gap = __any(x < x1 && pg >= a.n_pages);
+                if (lane == 0) s_gap[u % 3] = gap;
+            };
+            // What a lane brings of a turn: of the keys piece `piece` of every eighth row, of the values that piece of the eight keys of an
+            // operand.  One sequence of loads for both (a branch around them would have to wait for them at its end).
+            u32x4 hold[8 * SETS];
+            const bool values = wave >= CREW, works = CREW == 2 || wave < 2;
+            const int in_crew = (wave % CREW) * 64 + lane, piece = values ? (lane >> 3) + 8 * (wave % CREW) : in_crew % LPR;
+            const int key0 = values ? ((lane & 7) >> 1) * 16 + (lane & 1) * 4 : in_crew / LPR;
+            auto key_of = [&](int q) { return key0 + (values ? (q >> 2) * 8 + (q & 3) : q * 8); };
+            auto ask = [&](int u) {               // turn u's rows into registers (of a key that is none any row will do)
+                const int64_t* off = s_off + u % 3 * 64;
+                const T* base = values ? vbase : kbase;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const T* row = base + max(off[key_of(q)], (int64_t)0);
+#pragma unroll
+                    for (int st = 0; st < SETS; ++st) hold[st * 8 + q] = load16(row + min((piece + 16 * st) * 8, D - 8));
+                }
+            };
+            auto put = [&](int u) {               // and from there to LDS
+                char* buf = lds + (u & 1) * L::BUF;
+                if (!values) {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+#pragma unroll
+                        for (int st = 0; st < SETS; ++st)
+                            if (piece + 16 * st < NP) *reinterpret_cast<u32x4*>(buf + (key0 + q * 8) * L::KROW + (piece + 16 * st) * 16) = hold[st * 8 + q];
+                } else {
+                    const int xb = (int)x0 + u * 64;
+                    const bool look = xb < wg_lo || xb + 64 > min(wg_hi, x1) || __builtin_amdgcn_readfirstlane(s_gap[u % 3]);
+                    if (look) {
+                        unsigned odd = 0u;
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {
+                            const bool none = s_off[u % 3 * 64 + key_of(q)] < 0;
+#pragma unroll
+                            for (int st = 0; st < SETS; ++st)
+#pragma unroll
+                                for (int d = 0; d < 4; ++d) {
+                                    const unsigned w = none ? 0u : hold[st * 8 + q][d], bad = ((w & El<T>::ABS) + El<T>::STEP) & ~El<T>::ABS;
+                                    hold[st * 8 + q][d] = w & ~((bad - (bad >> 15)) | bad);
+                                    odd |= bad;
+                                }
+                        }
+                        if (odd) *s_odd = 1;
+                    }
+#pragma unroll
+                    for (int st = 0; st < SETS; ++st)
+                        if (piece + 16 * st < PIECES) {
+                            const u32x4 w[8] = {hold[st * 8], hold[st * 8 + 1], hold[st * 8 + 2], hold[st * 8 + 3], hold[st * 8 + 4], hold[st * 8 + 5], hold[st * 8 + 6], hold[st * 8 + 7]};
+                            char* at = buf + L::K + (piece + 16 * st) * 8 * L::VROW + (lane & 7) * 16;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) *reinterpret_cast<u32x4*>(at + e * L::VROW) = __builtin_bit_cast(u32x4, gather(w, e, f16()));
+                        }
+                }
+            };
+
+            __syncthreads();                      // the buffers of the turns before are free
+            if (wave == 0) { look_up(0, page_number(0)); if (turns > 1) look_up(1, page_number(1)); }
+            __syncthreads();
+            if (works) { ask(0); put(0); }
+            __syncthreads();
+            for (int u = 0; u < turns; ++u) {
+                const bool more = u + 1 < turns;
+                // (unconditionally, the last turn's over again at the end: see hold)
+                if (works) ask(min(u + 1, turns - 1));
+                const unsigned pg = page_number(u + 2);
+                const char* buf = lds + (u & 1) * L::BUF;
+                const int64_t* off = s_off + u % 3 * 64 + h * 4;
+                const bool gap = __builtin_amdgcn_readfirstlane(s_gap[u % 3]);
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) {
+                    const int xb = (int)x0 + u * 64 + sub * 32;
+                    if (xb >= min(any_hi, x1) || xb + 32 <= any_lo) continue;         // none of the wave's rows sees any of them
+                    f32x16 sc;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < NKS; ++ks)
+                        sc = Mfma32<T>::go(*reinterpret_cast<const vec*>(buf + (sub * 32 + c) * L::KROW + (ks * 2 + h) * 16), qf[ks], sc);
+                    if (xb + 32 > x1 || xb < all_lo || xb + 32 > all_hi || gap) {
+                        const int end = min(xhi, x1);
+                        const unsigned d0 = (unsigned)(xb + h * 4 - xlo), dn = (unsigned)(end > xlo ? end - xlo : 0);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) sc[r] = d0 + (r >> 2) * 8 + (r & 3) < dn ? sc[r] : -INFINITY;
+                        if (gap) {                // positions on no page are seen by nobody
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                if (off[sub * 32 + (r >> 2) * 8 + (r & 3)] < 0) sc[r] = -INFINITY;
+                        }
+                    }
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[r]);
+                    const float m_new = fmaxf(m, swap_halves_max(mx) * a.c_abs), base = m_new == -INFINITY ? 0.f : m_new;
+                    if (__any(m_new != m)) {
+                        const float alpha = __builtin_amdgcn_exp2f(m - base);
+                        l *= alpha;
+#pragma unroll
+                        for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
+                        m = m_new;
+                    }
+                    vec pf[2];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], a.c_abs, -base));
+                        l += p;
+                        pf[r >> 3][r & 7] = (T)p;
+                    }
+#pragma unroll
+                    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                        for (int dt = 0; dt < NDT; ++dt) {
+                            const vec vt = *reinterpret_cast<const vec*>(buf + L::K + (dt * 32 + c) * L::VROW + ((sub * 2 + s2) * 2 + h) * 16);
+                            acc[dt] = Mfma32<T>::go(vt, pf[s2], acc[dt]);
+                        }
+                }
+                if (works && more) put(u + 1);    // into the buffer of the turn before
+                if (wave == 0 && u + 2 < turns) look_up(u + 2, pg);
+                __syncthreads();
+            }
+        }
+
+        // ---- values that are no numbers -------------------------------------------------------------------------------------------
+        // They may sit in rows that some queries do not see, and 0 * NaN would have reached them: where a turn is masked at all they
+        // have left the operands.  If there were any, the queries that see their keys get them here, one key at a time.
+        if (__builtin_amdgcn_readfirstlane(*s_odd)) {
+            for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
+                const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n);
+                for (int x = (int)x0; x < x1; ++x) {
+                    const int xb = (int)x0 + (x - (int)x0) / 64 * 64;
+                    if (xb >= wg_lo && xb + 64 <= min(wg_hi, x1)) continue;
+                    const unsigned row = __builtin_amdgcn_readfirstlane(cache_row(a, s, t.kb + x));
+                    if (row == BAD) continue;
+                    const T *vp = vbase + cache_offset(a, row), *kp = kbase + cache_offset(a, row);
+                    bool odd = false;
+                    for (int d = lane; d < D; d += 64) odd |= !(fabsf((float)vp[d]) < INFINITY);
+                    if (!__any(odd)) continue;
+                    float dot = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < NKS; ++ks) {
+                        const vec kf = __builtin_bit_cast(vec, load16(kp + min((ks * 2 + h) * 8, D - 8)));
+                        vec q = qf[ks];
+                        asm volatile("" : "+v"(q));           // (or the queries are made single-precision for all keys at once: 128 registers)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) dot = fmaf((float)kf[e], (float)q[e], dot);
+                    }
+                    dot += __shfl_xor(dot, 32);
+                    const float pk = __builtin_amdgcn_exp2f(fmaf(dot, a.c_abs, -m));
+                    const bool take = x >= xlo && x < xhi;
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int pc = dt * 4 + (r >> 2), e = h * 4 + (r & 3);
+                            const float v = pc < NP ? (float)vp[min(pc * 8, D - 8) + e] : 0.f;
+                            if (take && !(fabsf(v) < INFINITY)) acc[dt][r] += pk * v;
+                        }
+                }
+            }
+        }
+
+        // ---- states out ---------------------------------------------------------------------------------------------------------
+        const int64_t tok = s.t0 + qi;
+        const float sum = l + __shfl_xor(l, 32);
+        const float mine = n_act > 1 ? 1.f : sum != 0.f ? 1.f / sum : 0.f;
+        if (R < t.rows) {
+            if (n_act > 1 && h == 0) {
+                float* o = a.ml + ((tok * a.n_head + head) * a.splits + split) * 2;
+                o[0] = m; o[1] = sum;
+            }
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const int pc = dt * 4 + r4;
+                    if (pc >= NP) continue;
+                    const int at = min(pc * 8, D - 8) + h * 4;
+                    if (n_act > 1) {
+                        float* o = a.part + (((tok * a.n_head + head) * a.splits + split) * (int64_t)D + at);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[k] = acc[dt][r4 * 4 + k];
+                    } else {
+                        T* o = (T*)a.out + tok * a.o_row + (int64_t)head * a.o_head + at;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[k] = (T)(acc[dt][r4 * 4 + k] * mine);
+                    }
+                }
+        }
+    }
+}
+
 // Joins the splits' states of rows that were split: a wave 64 channels of a row of a tile, four a lane, a quarter of the splits each
 // sixteen lanes; their weights one a lane.  (A wave a row left 16 waves to read 32 states of 480 channels: 19 us, now 5.)
 template <typename T>
@@ -550,7 +853,7 @@ __global__ __launch_bounds__(64) void attn_paged_join_kernel(const Args a, int t
         const Tile t = tile_of(a, s, tile);
         const int n_act = active_splits(a, t.n);
         if (n_act < 2) continue;
-        for (int R = t.row0 + wr; R < min(t.row0 + 16, t.rows); R += tile_rows) {
+        for (int R = t.row0 + wr; R < min(t.row0 + a.tr, t.rows); R += tile_rows) {
             const int i = (int)jb_div(R, a.group);
             const int64_t tok = s.t0 + t.j0 + i * t.js;
             const int h = kvh * a.G + (R - i * a.G);
@@ -581,32 +884,42 @@ __global__ __launch_bounds__(64) void attn_paged_join_kernel(const Args a, int t
     }
 }
 
-struct Plan { int64_t tiles, range; int splits; unsigned chunk; };
+struct Plan { int64_t tiles, range; int tr, splits; unsigned chunk; };       // tr: rows of a tile, 16 the rows kernel's, 128 the chunks'
 Plan plan_of(const jb_attn_paged_args* p) {
     Plan w;
-    const int64_t G = p->n_head / p->n_kv_head, bc = p->block_ctx;
+    const int64_t G = p->n_head / p->n_kv_head, bc = p->block_ctx, rows = p->max_q * G, streams = (int64_t)p->n_kv_head * p->n_seq;
+    w.tr = 16;
+    if (p->dtype != JB_F32 && p->attn_func != JB_ATTN_TRANSPOSE_BLOCK && p->d_head <= 256 && rows >= 64)
+        w.tr = 128;
     if (p->attn_func == JB_ATTN_TRANSPOSE_BLOCK) w.tiles = (int64_t)(p->max_q < bc ? p->max_q : bc) * (((p->max_q + bc - 1) / bc * G + 15) / 16);
-    else w.tiles = (p->max_q * G + 15) / 16;
+    else w.tiles = (rows + w.tr - 1) / w.tr;
     // keys that a tile walks at most
     w.range = p->max_len;
-    if (p->attn_func == JB_ATTN_BLOCK || p->attn_func == JB_ATTN_PREV_BLOCK) w.range = bc + 16 / G + 15;
+    if (p->attn_func == JB_ATTN_BLOCK || p->attn_func == JB_ATTN_PREV_BLOCK) w.range = bc + w.tr / G + 15;
     else if (p->attn_func == JB_ATTN_TRANSPOSE_BLOCK) w.range = (p->max_len + bc - 1) / bc;
-    else if (p->window) w.range = (int64_t)p->window + 16 / G + 15;
+    else if (p->window) w.range = (int64_t)p->window + w.tr / G + 15;
     if (w.range > p->max_len) w.range = p->max_len;
-    const int64_t wgs = w.tiles * p->n_kv_head * p->n_seq;
+    const int64_t wgs = w.tiles * streams;
     w.splits = 1; w.chunk = 0x7fffffff;
+    int64_t chunk = 0;
     // Few tiles: the keys are split, so that every compute unit has two workgroups.  A workgroup costs some 5 us before its first keys
     // are there, so its turn is 256 keys at least (16 sequences of 4096-8192 keys under one head of 480: 43 us; 512 keys: 55, 128: 58) -- a
     // launch too small to fill the chip even so takes 64 (300 keys: 17 us against 32) -- and 2048 at most, which evens out
     // sequences of different lengths (64 of 511-8192 keys: 261 us against 267 unsplit).
-    if (wgs < 1024 && w.range > 64) {
-        int64_t chunk = (wgs * w.range / 512 + 127) / 128 * 128;
+    if (w.tr == 16 && wgs < 1024 && w.range > 64) {
+        chunk = (wgs * w.range / 512 + 127) / 128 * 128;
         if (chunk > 2048) chunk = 2048;
         if (chunk < 256) chunk = wgs * w.range <= 64 * 256 ? 64 : 256;
+    }
+    // chunks: their turns are long enough from 512 keys on (24 tiles that hold rows, 5000 keys: 149 us; unsplit 236; aimed at 512 or 2048
+    // workgroups instead of 1024: 165, 185)
+    if (w.tr > 16 && wgs < 1024 && w.range > 512) {
+        chunk = (wgs * w.range / 1024 + 127) / 128 * 128;
+        if (chunk < 512) chunk = 512;
+    }
+    if (chunk) {
         if ((w.range + chunk - 1) / chunk > 64) chunk = ((w.range + 63) / 64 + 127) / 128 * 128;      // the join holds 64 states
-        w.splits = (int)((w.range + chunk - 1) / chunk);
-        w.chunk = (unsigned)chunk;
-        if (w.splits < 2) { w.splits = 1; w.chunk = 0x7fffffff; }
+        if (w.range > chunk) { w.splits = (int)((w.range + chunk - 1) / chunk); w.chunk = (unsigned)chunk; }
     }
     return w;
 }
@@ -641,6 +954,19 @@ template <typename T, int NC> void launch_rows(const Args& k, int64_t wgs, hipSt
     else attn_paged_rows_kernel<T, NC, false><<<(unsigned)wgs, Shape<T, NC>::WAVES * 64, 0, s>>>(k);
 }
 
+template <typename T, int DP> int launch_chunk_of(const Args& k, int64_t wgs, hipStream_t s) {
+    constexpr int bytes = ChunkLds<DP>::ALL;
+    static const hipError_t ready = hipFuncSetAttribute((const void*)attn_paged_chunk_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    JB_HIP(ready);
+    attn_paged_chunk_kernel<T, DP><<<(unsigned)wgs, 256, bytes, s>>>(k);
+    return JB_OK;
+}
+template <typename T> int launch_chunk(const Args& k, int64_t wgs, hipStream_t s) {
+    return k.D <= 64 ? launch_chunk_of<T, 64>(k, wgs, s) : k.D <= 128 ? launch_chunk_of<T, 128>(k, wgs, s)
+           : k.D <= 160 ? launch_chunk_of<T, 160>(k, wgs, s) : launch_chunk_of<T, 256>(k, wgs, s);
+}
+template <> int launch_chunk<float>(const Args&, int64_t, hipStream_t) { return JB_ERR_UNSUPPORTED; }        // (never asked for: plan_of)
+
 }  // namespace
 
 extern "C" int64_t jb_attn_paged_workspace(const jb_attn_paged_args* a) {
@@ -672,10 +998,11 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     while ((1 << k.page_shift) < a->page_size) ++k.page_shift;
     k.n_tokens = a->n_tokens; k.n_seq = a->n_seq; k.n_head = a->n_head; k.n_kv = a->n_kv_head; k.G = a->n_head / a->n_kv_head; k.D = a->d_head;
     k.func = a->attn_func; k.bc = a->block_ctx > 0 ? a->block_ctx : 1; k.window = a->window;
-    k.tiles = (int)w.tiles; k.splits = w.splits; k.chunk = w.chunk;
+    k.tr = w.tr; k.tiles = (int)w.tiles; k.splits = w.splits; k.chunk = w.chunk;
     k.c = a->scale * 1.44269504088896340736f;
+    k.c_abs = fmaxf(fabsf(k.c), 1e-30f);
     // (a lane's offset inside a 16-row half is 32 bits wide)
-    k.aligned = a->page_size % 16 == 0 && a->attn_func != JB_ATTN_TRANSPOSE_BLOCK && a->row_stride <= 0x7fffffff / 64 - 512;
+    k.aligned = w.tr == 16 && a->page_size % 16 == 0 && a->attn_func != JB_ATTN_TRANSPOSE_BLOCK && a->row_stride <= 0x7fffffff / 64 - 512;
     const int64_t inner = w.tiles == 1 ? k.n_kv : w.tiles, groups = wgs * w.splits / inner;
     JB_REQUIRE((groups + 8) * inner <= 0x7fffffff, "grid too large");
     k.groups = (unsigned)groups; k.by_die = w.tiles == 1 ? groups >= 8 : k.n_kv % 8 == 0;
@@ -690,7 +1017,8 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     JB_REQUIRE(w.splits == 1 || wgs * tile_rows <= 0x7fffffff, "grid too large");
 #define JB_ROWS(T, CH)                                                            \
     do {                                                                          \
-        if (a->d_head <= 128) launch_rows<T, 128 / CH>(k, grid, s);               \
+        if (w.tr > 16) { const int rc2 = launch_chunk<T>(k, grid, s); if (rc2) return rc2; } \
+        else if (a->d_head <= 128) launch_rows<T, 128 / CH>(k, grid, s);               \
         else if (a->d_head <= 256) launch_rows<T, 256 / CH>(k, grid, s);          \
         else launch_rows<T, 512 / CH>(k, grid, s);                                \
         JB_CHECK_LAUNCH();                                                        \
