@@ -9,6 +9,13 @@
 // from an exponential in double precision (2^18 of them sum to 2^62), so partial sums are exact whoever adds them, and a comparison
 // with a border has the error of the weights alone, 2^-45 of the largest.  In single precision the sums of a row of 10^5 likely
 // tokens are off by some 10^-7 of the total, and one draw in a thousand would differ from the definition's.
+//
+// One workgroup a row, one launch: the largest logit; a histogram of 2048 bins over the 32 nats that weigh anything, in counts and
+// weights; the bin in which k or p is crossed, and among its few entries the last kept one; the kept weights by tiles of consecutive
+// indices; the tile that u falls into.  A row of 128000 16-bit logits is 256 KB, which its die's L2 keeps for the passes after the
+// first: memory's part of 256 such rows (65 MB) is 14 us.  Measured (256 x 128000 bf16, normal logits of deviation 2.5): no filter 39 us,
+// top-k 50 57, top-p 0.9 89, min-p 0.05 32, both 85; temperature 0 20.  What bounds it is the exponential in double precision of every
+// entry that is weighed (for 16-bit logits taken from a table in LDS instead: 122 -> 100 us with top-p) and the LDS atomics of the histogram.
 #include "paged.h"
 
 namespace {
@@ -62,31 +69,43 @@ template <typename T> __device__ __forceinline__ u32x4 load_row(const T* row, in
     }
     return v;
 }
-// f(logit, index) for the whole row, every thread its part: U 16-byte requests in flight
-template <typename T, int NT, typename F> __device__ __forceinline__ void each(const T* row, int n, F f) {
+// f(16 bytes, index of the first) for the whole row, every thread its part: U requests in flight while U others are worked on
+template <typename T, int NT, typename F> __device__ __forceinline__ void each_load(const T* row, int n, F f) {
     constexpr int E = Row<T>::E, STEP = NT * E, U = 16 / E;
+    u32x4 next[U];
+    auto ask = [&](int i) {
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+            if (i + q * STEP < n) next[q] = load_row(row, i + q * STEP, n);
+    };
+    ask(threadIdx.x * E);
     for (int i = threadIdx.x * E; i < n; i += U * STEP) {
         u32x4 v[U];
 #pragma unroll
-        for (int q = 0; q < U; ++q)
-            if (i + q * STEP < n) v[q] = load_row(row, i + q * STEP, n);
+        for (int q = 0; q < U; ++q) v[q] = next[q];
+        ask(i + U * STEP);
 #pragma unroll
         for (int q = 0; q < U; ++q)
-            if (i + q * STEP < n) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) f(Row<T>::get(v[q], e), i + q * STEP + e);
-            }
+            if (i + q * STEP < n) f(v[q], i + q * STEP);
     }
+}
+// f(logit, index)
+template <typename T, int NT, typename F> __device__ __forceinline__ void each(const T* row, int n, F f) {
+    each_load<T, NT>(row, n, [&](u32x4 v, int i) {
+#pragma unroll
+        for (int e = 0; e < Row<T>::E; ++e) f(Row<T>::get(v, e), i + e);
+    });
 }
 
 // order-preserving integers of floats
 __device__ __forceinline__ unsigned key_of(float x) { const unsigned b = __float_as_uint(x); return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u); }
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
-struct Weigh {
+template <typename T, bool TABLE> struct Weigh {
     float mx, bins;                                   // largest logit; bins per unit of logit
     double c, md;                                     // 32 / (T ln 2); the largest logit
     const double* tab;                                // EXP2_32 in LDS: 32 entries, one pair of banks each
+    const double* keys;                               // a table of the weights themselves (see real), or NULL
     // how far below the largest, in bins; NB - 1: weighs nothing
     __device__ __forceinline__ float depth(float x) const { return x == mx ? 0.f : fminf((mx - x) * bins, (float)(NB - 1)); }
     __device__ __forceinline__ int bin(float x) const { return (int)depth(x); }
@@ -105,9 +124,9 @@ struct Weigh {
     }
     // 2^44 exp((x - max) / T) in double: z = n + f in 32nds of an octave; 2^(f / 32) by the Taylor series of the exponential to the
     // fourth power (f <= 1/2: the next term is 1.2e-12 of the weight), 2^(n / 32) from the table and the exponent field.  n by
-    // adding and taking away 1.5 2^52, in whose low word it stands meanwhile.  For x within RANGE T of the largest.
-    __device__ __forceinline__ double real(float x) const {
-        const double z = x == mx ? 0.0 : ((double)x - md) * c, t = z + 6755399441055744.0, f = z - (t - 6755399441055744.0);
+    // adding and taking away 1.5 2^52, in whose low word it stands meanwhile.
+    __device__ __forceinline__ double power(double z) const {
+        const double t = z + 6755399441055744.0, f = z - (t - 6755399441055744.0);
         double p = fma(f, L4, L3);
         p = fma(p, f, L2);
         p = fma(p, f, L1);
@@ -115,6 +134,39 @@ struct Weigh {
         const int n = (int)__double_as_longlong(t);
         const double w = p * tab[n & 31];
         return __hiloint2double(__double2hiint(w) + ((n >> 5) + 44) * 0x100000, __double2loint(w));
+    }
+    __device__ __forceinline__ double direct(float x) const { return power(x == mx ? 0.0 : ((double)x - md) * c); }
+    // Logits of 16 bits are few: those of 2^-10 .. 2^7 in magnitude, by their first 7 fraction bits, have a table in LDS (17 octaves of two
+    // signs), and the three further bits of a half another, by which the first is multiplied.  A logit has one weight, here as there.
+    static constexpr int OCTAVES = 17, FIRST = 127 - 10, KEYS = OCTAVES * 128, REST = OCTAVES * 8;
+    __device__ __forceinline__ double real(float x) const {
+        if constexpr (TABLE) {
+            const unsigned b = __float_as_uint(x), m = b & 0x7fffffffu, i = (m >> 16) - (FIRST << 7);
+            if (keys && i < (unsigned)KEYS) {
+                double w = keys[i + (b >> 31) * KEYS];
+                if constexpr (__is_same(T, f16)) {
+                    w *= keys[2 * KEYS + (m >> 13 & 7u) + (i >> 7) * 8 + (b >> 31) * REST];
+                    w = x == mx ? W1 : w;
+                }
+                return w;
+            }
+        }
+        return direct(x);
+    }
+    // (entries that no logit of this row has may lie far above or below its largest: their powers are cut off, not their products)
+    template <int NT> __device__ __forceinline__ void fill(double* table) {
+        auto far = [&](double z) { return power(fmin(fmax(z, -30000.0), 30000.0)); };
+        for (int i = threadIdx.x; i < 2 * KEYS; i += NT) {
+            const float x = __uint_as_float(((unsigned)(i % KEYS) + (FIRST << 7)) << 16 | (i >= KEYS ? 0x80000000u : 0u));
+            table[i] = x == mx ? W1 : far(((double)x - md) * c);
+        }
+        if constexpr (__is_same(T, f16))
+            for (int i = threadIdx.x; i < 2 * REST; i += NT) {
+                const int k = i % REST;
+                const double d = (double)(k & 7) * __uint_as_float((unsigned)((k >> 3) + FIRST - 10) << 23);
+                table[2 * KEYS + i] = far((i >= REST ? -d : d) * c) * (1.0 / W1);
+            }
+        keys = table;
     }
     // a whole number in the low bits of the sum with 2^52: rounded to nearest
     static __device__ __forceinline__ u64 whole(double w) { return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull; }
@@ -146,6 +198,7 @@ struct Shared {
     u64 w[CAP];                                       // ... and weights
     u64 tile[MAX_BINS / 1024];                        // kept weight of 256 E consecutive entries
     double tab[32];
+    unsigned lo_key, hi_key;                          // of the border bin's logits
     u64 part[16];
     u64 border;                                       // place of the last kept entry
     u64 before_w, before_n;                           // in front of the bin that a search has found
@@ -180,26 +233,18 @@ template <int NT> __device__ __forceinline__ void clear_bins(Shared& s) {
 // f(logit) is true for the entries that count: add(bin, weight) for each.  Where a whole wave's 16 bytes hold one value (a mask's, over
 // half the vocabulary), whose additions would queue up at one address, it enters once, for all of them.
 template <typename T, int NT, typename F> __device__ __forceinline__ void each_run(const T* row, int n, F f) {
-    constexpr int E = Row<T>::E, STEP = NT * E, U = 16 / E;
-    for (int i = threadIdx.x * E; i < n; i += U * STEP) {
-        u32x4 v[U];
+    constexpr int E = Row<T>::E;
+    each_load<T, NT>(row, n, [&](u32x4 v, int) {
+        const unsigned one = __builtin_amdgcn_readfirstlane(v[0]);
+        const bool same = v[0] == one && v[1] == one && v[2] == one && v[3] == one && (E == 4 || (one >> 16) == (one & 0xffffu));
+        const u64 all = __ballot(1);
+        if (__ballot(same) == all) {
+            if ((all & ((1ull << (threadIdx.x & 63)) - 1)) == 0) f(Row<T>::get(v, 0), (unsigned)__popcll(all) * E);
+        } else {
 #pragma unroll
-        for (int q = 0; q < U; ++q)
-            if (i + q * STEP < n) v[q] = load_row(row, i + q * STEP, n);
-#pragma unroll
-        for (int q = 0; q < U; ++q) {
-            if (i + q * STEP >= n) continue;
-            const unsigned w = v[q][0], one = __builtin_amdgcn_readfirstlane(w);
-            const bool same = w == one && v[q][1] == one && v[q][2] == one && v[q][3] == one && (E == 4 || (one >> 16) == (one & 0xffffu));
-            const u64 all = __ballot(1);
-            if (__ballot(same) == all) {
-                if ((all & ((1ull << (threadIdx.x & 63)) - 1)) == 0) f(Row<T>::get(v[q], 0), (unsigned)__popcll(all) * E);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) f(Row<T>::get(v[q], e), 1u);
-            }
+            for (int e = 0; e < E; ++e) f(Row<T>::get(v, e), 1u);
         }
-    }
+    });
 }
 // The first bin at which the running count (COUNT) or weight exceeds `limit`; NB if none does.  s.before_*: the sums in front of it.
 template <int NT, bool COUNT> __device__ int crossing(u64 limit, Shared& s, bool weights_too = false) {
@@ -229,11 +274,11 @@ template <int NT, bool COUNT> __device__ int crossing(u64 limit, Shared& s, bool
 struct Found { u64 border, mass; };
 
 // Many entries in the bin (equal logits): by the digits of their places, which are all different.  Rare, hence a call.
-template <typename T, int NT, bool COUNT>
-__device__ __attribute__((noinline)) Found search_digits(const T* row, int n, const Weigh g, int which, u64 limit, bool with_mass, Shared& s) {
+template <typename T, int NT, bool COUNT, typename G>
+__device__ __attribute__((noinline)) Found search_digits(const T* row, int n, const G g, int which, u64 limit, bool with_mass, u64 start, Shared& s) {
     const float lo = g.below(which + 1), hi = g.below(which);
-    u64 prefix = 0, before = 0;
-    for (int d = 0; d < 5; ++d) {
+    u64 prefix = start, before = 0;                   // (start: the place of the bin's only value, without the index)
+    for (int d = start ? 3 : 0; d < 5; ++d) {
         __syncthreads();
         clear_bins<NT>(s);
         // 32 bits of the logit as 11, 11 and 10, 18 of the index as 9 and 9
@@ -249,7 +294,20 @@ __device__ __attribute__((noinline)) Found search_digits(const T* row, int n, co
             }
         };
         if (d < 3) each_run<T, NT>(row, n, [&](float x, unsigned times) { add(x, 0, times); });
-        else each<T, NT>(row, n, [&](float x, int i) { add(x, i, 1u); });
+        else if (d == 4) each<T, NT>(row, n, [&](float x, int i) { add(x, i, 1u); });
+        else {
+            // (the index's upper digit is the same for the entries of a load: they enter together)
+            unsigned times = 0;
+            u64 w = 0;
+            each<T, NT>(row, n, [&](float x, int i) {
+                if (x > lo && x <= hi && (place(x, 0) ^ prefix) >> 32 == 0) { ++times; w += g.whole(x); }
+                if ((i + 1) % Row<T>::E == 0 && times) {
+                    if (COUNT) atomicAdd(&s.count[i >> 9], times);
+                    if (with_mass || !COUNT) atomicAdd(&s.mass[i >> 9], w);
+                    times = 0; w = 0;
+                }
+            });
+        }
         __syncthreads();
         const int b = crossing<NT, COUNT>(limit, s, with_mass);
         // (none: everything of this prefix is kept -- its largest place stands for it)
@@ -262,34 +320,46 @@ __device__ __attribute__((noinline)) Found search_digits(const T* row, int n, co
     __syncthreads();
     return Found{prefix, before};
 }
-template <typename T, int NT, bool COUNT>
-__device__ __forceinline__ Found select(const T* row, int n, const Weigh& g, int which, u64 limit, bool with_mass, Shared& s) {
-    if (threadIdx.x == 0) { s.n = 0; s.border = 0; }
+template <typename T, int NT, bool COUNT, typename G>
+__device__ __forceinline__ Found select(const T* row, int n, const G& g, int which, u64 limit, bool with_mass, Shared& s) {
+    if (threadIdx.x == 0) { s.n = 0; s.border = 0; s.lo_key = ~0u; s.hi_key = 0; }
     __syncthreads();
     const float lo = g.below(which + 1), hi = g.below(which);       // the bin's logits: lo < x <= hi
     each<T, NT>(row, n, [&](float x, int i) {
         if (x > lo && x <= hi) {
             const unsigned at = atomicAdd(&s.n, 1u);
-            if (at < CAP) { s.at[at] = place(x, i); s.w[at] = g.whole(x); }
+            if (at < CAP) s.at[at] = place(x, i);
+            else if (at == CAP) s.hi_key = key_of(x + 0.0f);
         }
     });
     __syncthreads();
     const unsigned m = s.n;
-    if (m > CAP) return search_digits<T, NT, COUNT>(row, n, g, which, limit, with_mass, s);
-    // entry against entry
+    if (m > CAP) {
+        // one value only (the rule, with so many)?  Then its index alone is looked for.
+        const float one = of_key(s.hi_key);
+        bool other = false;
+        each<T, NT>(row, n, [&](float x, int) { other |= x > lo && x <= hi && x != one; });
+        if (other) s.lo_key = 0;
+        __syncthreads();
+        return search_digits<T, NT, COUNT>(row, n, g, which, limit, with_mass, s.lo_key ? place(one, 0) : 0, s);
+    }
+    if (!COUNT || with_mass) {
+        for (unsigned t = threadIdx.x; t < m; t += NT) s.w[t] = g.whole(of_key(~(unsigned)(s.at[t] >> 32)));
+        __syncthreads();
+    }
+    // entry against entry: one to a wave, the others over its lanes (one to a thread took 65 ns for each other entry)
+    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 sum = 0;
-    for (unsigned t = threadIdx.x; t < m; t += NT) {
+    for (unsigned t = wave; t < m; t += NT / 64) {
         const u64 me = s.at[t];
-        unsigned nb = 0;
-        u64 wb = 0;
-        if (COUNT) {
-#pragma unroll 8
-            for (unsigned j = 0; j < m; ++j) nb += s.at[j] < me;
-        } else {
-#pragma unroll 4
-            for (unsigned j = 0; j < m; ++j) wb += s.at[j] < me ? s.w[j] : 0;
+        u64 before = 0;
+        for (unsigned j = lane; j - lane < m; j += 64) {
+            const bool less = j < m && s.at[j] < me;
+            if (COUNT) before += __popcll(__ballot(less));
+            else before += less ? s.w[j] : 0;
         }
-        if ((COUNT ? nb : wb) <= limit) { atomicMax(&s.border, me); sum += s.w[t]; }
+        if (!COUNT) before = wave_sum(before);
+        if (lane == 0 && before <= limit) { atomicMax(&s.border, me); if (!COUNT || with_mass) sum += s.w[t]; }
     }
     Found f;
     block_scan<NT>(sum, s, &f.mass);
@@ -300,6 +370,7 @@ __device__ __forceinline__ Found select(const T* row, int n, const Weigh& g, int
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_filtered_kernel(const Args a) {
     constexpr int E = Row<T>::E;
+    constexpr bool TABLE = E == 8 && NT == 1024;      // (4352 weights to begin with: not for a short row's sake)
     __shared__ Shared s;
     const int n = a.bins, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r = blockIdx.x;
@@ -326,17 +397,26 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const Args a) {
     }
     const int k = a.top_k ? a.top_k[r] : a.top_k_all;
     const float p = a.top_p ? a.top_p[r] : a.top_p_all;
-    Weigh g;
+    Weigh<T, TABLE> g;
     g.mx = top;
     g.c = 1.0 / (LN2_32 * (double)temp);
     g.md = (double)g.mx;
     g.bins = (float)fmin((double)NB / RANGE / (double)temp, 1e30);
     g.tab = s.tab;
+    g.keys = nullptr;
     const double least = fmin((double)(a.min_p ? a.min_p[r] : a.min_p_all), 1.0) * W1;
     const bool by_k = k > 0 && k < n, by_p = p > 0.f && p < 1.f;
     u64 border = ~0ull;
     // entries up to this logit weigh nothing.  (Of a row whose largest logit is infinite only its equals weigh anything.)
     const float zero = g.below(NB - 1);
+    if constexpr (TABLE) {
+        // where most entries are weighed, and the temperature leaves the rests' powers within a double's range
+        __shared__ double keys[2 * (Weigh<T, TABLE>::KEYS + (__is_same(T, f16) ? Weigh<T, TABLE>::REST : 0))];
+        if (temp >= 0.002f && (by_p || !(by_k || least > 0.0))) {
+            g.template fill<NT>(keys);
+            __syncthreads();
+        }
+    }
 
     if (by_k || by_p) {
         clear_bins<NT>(s);
@@ -399,56 +479,50 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const Args a) {
     // what top-k and top-p have kept: x > cut, or x == cut and index <= last
     const float cut = border == ~0ull ? zero : of_key(~(unsigned)(border >> 32));
     const int last = border == ~0ull ? -1 : (int)(unsigned)border;
-    const bool few = border != ~0ull || least > 0.0;
     // (a little below what min-p leaves, in logits: the weight itself decides)
     float rough = zero;
     if (least > 0.0) {
         const float f = (float)((double)top + (double)temp * (log(least / W1) - 1e-3)) - fabsf(top) * 0x1p-22f;
         if (f > zero && f < top) rough = f;
     }
-    auto in = [&](float x, int i) { return x > rough && (x > cut || (x == cut && i <= last)); };
     auto weight = [&](float x) -> u64 {
         const double w = g.real(x);
-        return w >= least ? Weigh::whole(w) : 0;
+        return w >= least ? g.whole(w) : 0;
     };
+    const bool everything = border == ~0ull && !(least > 0.0);
+    // the smallest logit to look at (the one above `zero`, which weighs nothing)
+    const float edge = everything ? of_key(key_of(zero) + 1) : fmaxf(cut, rough);
+    auto in = [&](float x, int i) { return x > rough && (x > cut || (x == cut && i <= last)); };
+    u32x4 next[4];
+    auto ask = [&](int t) {
+        const int i = t * TILE + lane * E;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (i + q * 64 * E < n) next[q] = load_row(row, i + q * 64 * E, n);
+    };
+    ask(wave);
     for (int t = wave; t < tiles; t += NT / 64) {
         const int i = t * TILE + lane * E;
         u32x4 v[4];
         u64 w = 0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (i + q * 64 * E < n) v[q] = load_row(row, i + q * 64 * E, n);
-        if (few) {
-            // most tiles of a short list hold nothing of it
-            float most = -INFINITY;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (i + q * 64 * E < n) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) most = fmaxf(most, Row<T>::get(v[q], e));
-                }
-            if (__any(most >= cut && most > rough)) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (i + q * 64 * E < n) {
-#pragma unroll
-                        for (int e = 0; e < E; ++e) {
-                            const float x = Row<T>::get(v[q], e);
-                            if (in(x, i + q * 64 * E + e)) w += weight(x);
-                        }
-                    }
-            }
-        } else {
+        for (int q = 0; q < 4; ++q) v[q] = next[q];
+        ask(t + NT / 64);
+        auto each_kept = [&](auto f) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 if (i + q * 64 * E < n) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
                         const float x = Row<T>::get(v[q], e);
-                        if (x > zero) w += g.whole(x);
+                        if (x >= edge) f(x, i + q * 64 * E + e);
                     }
                 }
-        }
+        };
+        // (three forms: no filter 17 us of a row of 128000, the general one 24; top-k 8 with the single comparison in front, 14 without)
+        if (everything) each_kept([&](float x, int) { w += g.whole(x); });
+        else if (least > 0.0) each_kept([&](float x, int j) { if (in(x, j)) w += weight(x); });
+        else each_kept([&](float x, int j) { if (x > cut || j <= last) w += g.whole(x); });
         w = wave_sum(w);
         if (lane == 0) s.tile[t] = w;
     }
