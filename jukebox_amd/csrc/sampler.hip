@@ -14,8 +14,8 @@
 // weights; the bin in which k or p is crossed, and among its few entries the last kept one; the kept weights by tiles of consecutive
 // indices; the tile that u falls into.  A row of 128000 16-bit logits is 256 KB, which its die's L2 keeps for the passes after the
 // first: memory's part of 256 such rows (65 MB) is 14 us.  Measured (256 x 128000 bf16, normal logits of deviation 2.5): no filter 39 us,
-// top-k 50 57, top-p 0.9 89, min-p 0.05 32, both 85; temperature 0 20.  What bounds it is the exponential in double precision of every
-// entry that is weighed (for 16-bit logits taken from a table in LDS instead: 122 -> 100 us with top-p) and the LDS atomics of the histogram.
+// top-k 50 56, top-p 0.9 84, both 85, min-p 0.05 33; temperature 0 20; two thirds of the entries equal, top-p 129.  What bounds it is the exponential in double precision of every
+// entry that is weighed (for 16-bit logits taken from a table in LDS instead: 120 -> 98 us with top-p when it came in) and the LDS atomics of the histogram.
 #include "paged.h"
 
 namespace {
@@ -273,94 +273,135 @@ template <int NT, bool COUNT> __device__ int crossing(u64 limit, Shared& s, bool
 // before -- and the bin's weight up to and with it.
 struct Found { u64 border, mass; };
 
-// Many entries in the bin (equal logits): by the digits of their places, which are all different.  Rare, hence a call.
+// The same among the entries of one value, by their index: entry number limit (COUNT) or limit / weight.  False: the logits in
+// (lo, hi] are not all of that value.  Rare (more equal logits than a list holds), hence a call.
 template <typename T, int NT, bool COUNT, typename G>
-__device__ __attribute__((noinline)) Found search_digits(const T* row, int n, const G g, int which, u64 limit, bool with_mass, u64 start, Shared& s) {
-    const float lo = g.below(which + 1), hi = g.below(which);
-    u64 prefix = start, before = 0;                   // (start: the place of the bin's only value, without the index)
-    for (int d = start ? 3 : 0; d < 5; ++d) {
+__device__ __attribute__((noinline)) bool search_index(const T* row, int n, const G g, float one, float lo, float hi, u64 limit, Shared& s, Found* f) {
+    constexpr int E = Row<T>::E;
+    const int lane = threadIdx.x & 63;
+    __syncthreads();
+    clear_bins<NT>(s);
+    bool other = false;
+    each_load<T, NT>(row, n, [&](u32x4 v, int i) {
+        // a wave's loads are 64 E consecutive entries from a multiple of as many on: of one 512
+        unsigned times = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float x = Row<T>::get(v, e);
+            times += __popcll(__ballot(x == one));
+            other |= x > lo && x <= hi && x != one;
+        }
+        if (lane == 0 && times) atomicAdd(&s.count[i >> 9], times);
+    });
+    if (other) s.lo_key = 0;
+    __syncthreads();
+    if (s.lo_key == 0) return false;
+    u64 total, mine = 0;
+    for (int b = threadIdx.x; b < NB; b += NT) mine += s.count[b];
+    block_scan<NT>(mine, s, &total);
+    const u64 w = g.whole(one), nth = min(COUNT ? limit : w ? limit / w : ~0ull, total - 1);
+    const int b = crossing<NT, true>(nth, s);
+    if (threadIdx.x < 64) {
+        unsigned left = (unsigned)(nth - s.before_n);
+        for (int c = 0; c < 8; ++c) {
+            const int i = b * 512 + c * 64 + lane;
+            const bool eq = i < n && (float)row[i] == one;
+            const u64 who = __ballot(eq);
+            if (eq && __popcll(who & ((1ull << lane) - 1)) == left) s.border = place(one, i);
+            const unsigned here = __popcll(who);
+            if (left < here) break;
+            left -= here;
+        }
+    }
+    __syncthreads();
+    f->border = s.border;
+    f->mass = (nth + 1) * w;
+    return true;
+}
+// More entries than the list holds: of one value, as a rule.  Of different ones the border's by its digits, 11, 11 and 10 bits of the
+// places, then its index.
+template <typename T, int NT, bool COUNT, typename G>
+__device__ __attribute__((noinline)) Found search_many(const T* row, int n, const G g, float lo, float hi, u64 limit, bool with_mass, Shared& s) {
+    Found f;
+    for (int i = threadIdx.x * Row<T>::E; i < n && *(volatile unsigned*)&s.hi_key == 0; i += NT * Row<T>::E) {
+        const u32x4 v = load_row(row, i, n);
+#pragma unroll
+        for (int e = 0; e < Row<T>::E; ++e) {
+            const float x = Row<T>::get(v, e);
+            if (x > lo && x <= hi) s.hi_key = key_of(x + 0.0f);
+        }
+    }
+    __syncthreads();
+    if (search_index<T, NT, COUNT>(row, n, g, of_key(s.hi_key), lo, hi, limit, s, &f)) return f;
+    u64 prefix = 0, before = 0;
+    for (int d = 0; d < 3; ++d) {
         __syncthreads();
         clear_bins<NT>(s);
-        // 32 bits of the logit as 11, 11 and 10, 18 of the index as 9 and 9
-        const int bits = d < 2 ? 11 : d == 2 ? 10 : 9, sh = d < 3 ? 64 - 11 * d - bits : 9 * (4 - d), top = sh + bits;
-        auto add = [&](float x, int i, unsigned times) {
+        const int bits = d < 2 ? 11 : 10, sh = 64 - 11 * d - bits, top = sh + bits;
+        each_run<T, NT>(row, n, [&](float x, unsigned times) {
             if (x > lo && x <= hi) {
-                const u64 p = place(x, i);
+                const u64 p = place(x, 0);
                 if (d == 0 || (p ^ prefix) >> (top & 63) == 0) {
                     const int b = (int)(p >> sh) & ((1 << bits) - 1);
                     if (COUNT) atomicAdd(&s.count[b], times);
                     if (with_mass || !COUNT) atomicAdd(&s.mass[b], g.whole(x) * times);
                 }
             }
-        };
-        if (d < 3) each_run<T, NT>(row, n, [&](float x, unsigned times) { add(x, 0, times); });
-        else if (d == 4) each<T, NT>(row, n, [&](float x, int i) { add(x, i, 1u); });
-        else {
-            // (the index's upper digit is the same for the entries of a load: they enter together)
-            unsigned times = 0;
-            u64 w = 0;
-            each<T, NT>(row, n, [&](float x, int i) {
-                if (x > lo && x <= hi && (place(x, 0) ^ prefix) >> 32 == 0) { ++times; w += g.whole(x); }
-                if ((i + 1) % Row<T>::E == 0 && times) {
-                    if (COUNT) atomicAdd(&s.count[i >> 9], times);
-                    if (with_mass || !COUNT) atomicAdd(&s.mass[i >> 9], w);
-                    times = 0; w = 0;
-                }
-            });
-        }
+        });
         __syncthreads();
         const int b = crossing<NT, COUNT>(limit, s, with_mass);
         // (none: everything of this prefix is kept -- its largest place stands for it)
-        if (b == NB) { prefix |= d == 0 ? ~0ull : (1ull << top) - 1; break; }
+        if (b == NB) { __syncthreads(); return Found{prefix | (d == 0 ? ~0ull : (1ull << top) - 1), before}; }
         prefix |= (u64)b << sh;
         limit -= COUNT ? s.before_n : s.before_w;
         before += s.before_w;
-        if (d == 4) before += s.mass[b];
     }
-    __syncthreads();
-    return Found{prefix, before};
+    const float one = of_key(~(unsigned)(prefix >> 32));
+    if (threadIdx.x == 0) s.lo_key = ~0u;
+    search_index<T, NT, COUNT>(row, n, g, one, INFINITY, INFINITY, limit, s, &f);
+    f.mass += before;
+    return f;
 }
 template <typename T, int NT, bool COUNT, typename G>
 __device__ __forceinline__ Found select(const T* row, int n, const G& g, int which, u64 limit, bool with_mass, Shared& s) {
     if (threadIdx.x == 0) { s.n = 0; s.border = 0; s.lo_key = ~0u; s.hi_key = 0; }
     __syncthreads();
     const float lo = g.below(which + 1), hi = g.below(which);       // the bin's logits: lo < x <= hi
-    each<T, NT>(row, n, [&](float x, int i) {
-        if (x > lo && x <= hi) {
-            const unsigned at = atomicAdd(&s.n, 1u);
-            if (at < CAP) s.at[at] = place(x, i);
-            else if (at == CAP) s.hi_key = key_of(x + 0.0f);
-        }
-    });
-    __syncthreads();
+    // (more than the list holds for sure: they are not put there one by one, which for 85000 equal ones took 30 us)
+    bool many = COUNT ? s.count[which] > CAP : s.mass[which] > g.whole(fminf(hi, g.mx)) * CAP;
+    if (!many) {
+        each<T, NT>(row, n, [&](float x, int i) {
+            if (x > lo && x <= hi) {
+                const unsigned at = atomicAdd(&s.n, 1u);
+                if (at < CAP) s.at[at] = place(x, i);
+            }
+        });
+        __syncthreads();
+        many = s.n > CAP;
+    }
+    if (many) return search_many<T, NT, COUNT>(row, n, g, lo, hi, limit, with_mass, s);
     const unsigned m = s.n;
-    if (m > CAP) {
-        // one value only (the rule, with so many)?  Then its index alone is looked for.
-        const float one = of_key(s.hi_key);
-        bool other = false;
-        each<T, NT>(row, n, [&](float x, int) { other |= x > lo && x <= hi && x != one; });
-        if (other) s.lo_key = 0;
-        __syncthreads();
-        return search_digits<T, NT, COUNT>(row, n, g, which, limit, with_mass, s.lo_key ? place(one, 0) : 0, s);
+    // Entry against entry: the others in as many parts as there are threads for, a thread an entry and a part (154 entries: 5 us; one
+    // part 10, an entry to a wave 8).  The sums take the histogram's place.
+    for (unsigned t = threadIdx.x; t < m; t += NT) {
+        if (!COUNT || with_mass) s.w[t] = g.whole(of_key(~(unsigned)(s.at[t] >> 32)));
+        s.mass[t] = 0;
     }
-    if (!COUNT || with_mass) {
-        for (unsigned t = threadIdx.x; t < m; t += NT) s.w[t] = g.whole(of_key(~(unsigned)(s.at[t] >> 32)));
-        __syncthreads();
-    }
-    // entry against entry: one to a wave, the others over its lanes (one to a thread took 65 ns for each other entry)
-    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    u64 sum = 0;
-    for (unsigned t = wave; t < m; t += NT / 64) {
+    __syncthreads();
+    const unsigned wide = (m + 63) & ~63u, parts = max(NT / max(wide, 1u), 1u), per = (m + parts - 1) / parts;
+    for (unsigned i = threadIdx.x; i < wide * parts; i += NT) {
+        const unsigned part = i / wide, t = i - part * wide, end = min((part + 1) * per, m);
+        if (t >= m) continue;
         const u64 me = s.at[t];
         u64 before = 0;
-        for (unsigned j = lane; j - lane < m; j += 64) {
-            const bool less = j < m && s.at[j] < me;
-            if (COUNT) before += __popcll(__ballot(less));
-            else before += less ? s.w[j] : 0;
-        }
-        if (!COUNT) before = wave_sum(before);
-        if (lane == 0 && before <= limit) { atomicMax(&s.border, me); if (!COUNT || with_mass) sum += s.w[t]; }
+#pragma unroll 4
+        for (unsigned j = part * per; j < end; ++j) before += s.at[j] < me ? (COUNT ? 1 : s.w[j]) : 0;
+        atomicAdd(&s.mass[t], before);
     }
+    __syncthreads();
+    u64 sum = 0;
+    for (unsigned t = threadIdx.x; t < m; t += NT)
+        if (s.mass[t] <= limit) { atomicMax(&s.border, s.at[t]); if (!COUNT || with_mass) sum += s.w[t]; }
     Found f;
     block_scan<NT>(sum, s, &f.mass);
     f.border = s.border;

@@ -208,3 +208,31 @@ def test_in_a_graph(H):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_settings_as_large_as_they_may_be(H):
+    x, u = logits(4, 500, "f32", 31)
+    u = u.cuda()
+    want = H.sample_filtered(x, u)
+    for k in (500, 2 ** 31 - 1, 2 ** 40, -1, -2 ** 40):          # all of them, or off
+        assert torch.equal(H.sample_filtered(x, u, top_k=k), want)
+    assert torch.equal(H.sample_filtered(x, u, top_p=7.0), want) and torch.equal(H.sample_filtered(x, u, min_p=-3.0), want)
+    assert torch.equal(H.sample_filtered(x, u, min_p=9.0), x.argmax(1)) and torch.equal(H.sample_filtered(x, u, top_k=1), x.argmax(1))
+    assert H.sample_filtered(x[:0], u[:0]).numel() == 0
+    assert H.sample_filtered(x, u, temp=math.inf).min() >= 0
+
+
+def test_two_streams_at_once(H):
+    (x, u), (y, v) = logits(64, 128000, "bf16", 32), logits(300, 2048, "f32", 33)
+    u, v = u.cuda(), v.cuda()
+    want = [H.sample_filtered(x, u, 0.9, 50, 0.9), H.sample_filtered(y, v, 1.0, 0, 0.9)]
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        with torch.cuda.stream(s):
+            outs[0].append(H.sample_filtered(x, u, 0.9, 50, 0.9))
+        with torch.cuda.stream(t):
+            outs[1].append(H.sample_filtered(y, v, 1.0, 0, 0.9))
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, o) for w, os in zip(want, outs) for o in os)
