@@ -324,7 +324,7 @@ int jb_vq_argmin(const float* x, const float* xk, const float* codebook, int64_t
  * holds (the last is position lens[i] - 1) -- over its pages.  Replaces what jb_attn_decode / jb_attn_prefill do on a cache of one
  * fixed length per sample (FactoredAttention.forward(sample=True), jukebox/transformer/factored_attention.py:82-193,289-301).
  * Rows cu_q[i] .. cu_q[i+1]-1 of q [n_tokens][n_head][d_head] are sequence i's; rows outside every sequence are neither read
- * nor written.  n_head / n_kv_head consecutive query heads share a key / value head.  A query without a visible key (block 0
+ * nor written; out overlaps no input.  n_head / n_kv_head consecutive query heads share a key / value head.  A query without a visible key (block 0
  * of the prev pattern, a length below the number of queries) gives zeros; a masked key or value may hold anything, NaN too;
  * positions whose table entry is no page number are masked.  Patterns 0-3; `window` (dense only, 0 = off): the query at p sees
  * positions p - window + 1 .. p.  Strides in elements, channels contiguous; k and v share them.  Softmax in fp32; 16-bit

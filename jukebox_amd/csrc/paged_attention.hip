@@ -62,10 +62,11 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int i) {
     s.table = a.table + (int64_t)i * a.table_stride;
     return s;
 }
+__device__ __forceinline__ int times(int n, int bc) { return n > 0 ? (n - 1) / bc + 1 : 0; }      // ceil(n / bc), bc as large as it may be
 __device__ __forceinline__ int tiles_of(const Args& a, int nq) {
     if (a.func != JB_ATTN_TRANSPOSE_BLOCK) return (int)(((int64_t)nq * a.G + a.tr - 1) / a.tr);
     const int cls = min(a.bc, nq);
-    return cls == 0 ? 0 : cls * (int)(((int64_t)((nq + a.bc - 1) / a.bc) * a.G + a.tr - 1) / a.tr);
+    return cls * (int)(((int64_t)times(nq, a.bc) * a.G + a.tr - 1) / a.tr);
 }
 // Row r of a tile is token j0 + i * js of the chunk, i = (row0 + r) / G, head (row0 + r) % G; the keys that any of its rows
 // may see sit at positions kb + x * ks, x < n.
@@ -73,9 +74,9 @@ struct Tile { int j0, js, row0, rows, kb, ks, n; };      // rows: rows of this t
 __device__ __forceinline__ Tile tile_of(const Args& a, const Seq& s, int tile) {
     Tile t;
     if (a.func == JB_ATTN_TRANSPOSE_BLOCK) {             // one residue class of positions modulo bc
-        const int per = (int)(((int64_t)((s.nq + a.bc - 1) / a.bc) * a.G + a.tr - 1) / a.tr);
+        const int per = (int)(((int64_t)times(s.nq, a.bc) * a.G + a.tr - 1) / a.tr);
         t.j0 = tile / per; t.js = a.bc; t.row0 = (tile % per) * a.tr;
-        t.rows = (s.nq - t.j0 + a.bc - 1) / a.bc * a.G;
+        t.rows = times(s.nq - t.j0, a.bc) * a.G;
     } else {
         t.j0 = 0; t.js = 1; t.row0 = tile * a.tr; t.rows = s.nq * a.G;
     }
@@ -956,8 +957,13 @@ template <typename T, int NC> void launch_rows(const Args& k, int64_t wgs, hipSt
 
 template <typename T, int DP> int launch_chunk_of(const Args& k, int64_t wgs, hipStream_t s) {
     constexpr int bytes = ChunkLds<DP>::ALL;
-    static const hipError_t ready = hipFuncSetAttribute((const void*)attn_paged_chunk_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    JB_HIP(ready);
+    static bool configured[64] = {};                  // per device (a call that is made twice does no harm)
+    int dev = 0;
+    JB_HIP(hipGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        JB_HIP(hipFuncSetAttribute((const void*)attn_paged_chunk_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
     attn_paged_chunk_kernel<T, DP><<<(unsigned)wgs, 256, bytes, s>>>(k);
     return JB_OK;
 }

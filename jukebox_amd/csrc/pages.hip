@@ -409,7 +409,7 @@ extern "C" int jb_kv_write(const jb_kv_write_args* a, void* stream) {
 }
 
 extern "C" int jb_pages_extend(const jb_page_table* t, const int* cu_new, int n_tokens, int64_t* slots, int* work, int* status, void* stream) {
-    JB_REQUIRE(t && t->table && t->lens && t->ref && cu_new && work && status && (slots || n_tokens == 0), "null pointer");
+    JB_REQUIRE(t && (t->n_seq == 0 || (t->table && t->lens)) && t->ref && cu_new && work && status && (slots || n_tokens == 0), "null pointer");
     JB_REQUIRE(t->n_seq >= 0 && t->max_pages > 0 && t->n_pages > 0 && t->page_size > 0 && n_tokens >= 0, "bad dims");
     JB_REQUIRE(t->table_stride >= t->max_pages || t->n_seq < 2, "rows of the table overlap");
     JB_REQUIRE((int64_t)t->n_pages * t->page_size <= 0x7fffffff, "more than 2^31 cache rows");
@@ -428,7 +428,7 @@ extern "C" int jb_pages_extend(const jb_page_table* t, const int* cu_new, int n_
 }
 
 extern "C" int jb_pages_free(const jb_page_table* t, const int* rows, int n_rows, int* status, void* stream) {
-    JB_REQUIRE(t && t->table && t->lens && t->ref && status && (rows || n_rows == 0), "null pointer");
+    JB_REQUIRE(t && (t->n_seq == 0 || (t->table && t->lens)) && t->ref && status && (rows || n_rows == 0), "null pointer");
     JB_REQUIRE(t->n_seq >= 0 && t->max_pages > 0 && t->n_pages > 0 && n_rows >= 0, "bad dims");
     JB_REQUIRE(t->table_stride >= t->max_pages || t->n_seq < 2, "rows of the table overlap");
     JB_REQUIRE(t->n_seq <= MAX_SEQS && n_rows <= t->n_seq, "more rows than the table has, or a table of more than 131072");
@@ -453,7 +453,7 @@ extern "C" int jb_pages_copy(const jb_page_pools* p, const int* src, const int* 
 }
 
 extern "C" int jb_pages_fork(const jb_page_table* t, const jb_page_pools* p, const int* src, const int* dst, int n_pairs, int* work, int* status, void* stream) {
-    JB_REQUIRE(t && t->table && t->lens && t->ref && work && status && (n_pairs == 0 || (src && dst)), "null pointer");
+    JB_REQUIRE(t && (t->n_seq == 0 || (t->table && t->lens)) && t->ref && work && status && (n_pairs == 0 || (src && dst)), "null pointer");
     const int rc = pools_fit(__func__, p);
     if (rc) return rc;
     JB_REQUIRE(t->n_seq >= 0 && t->max_pages > 0 && t->n_pages > 0 && t->page_size > 0 && n_pairs >= 0 && t->n_pages == p->n_pages, "bad dims");

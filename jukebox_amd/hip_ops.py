@@ -305,6 +305,7 @@ def attn_prefill(func, q, kcache, vcache, n_head, block_ctx, t0):
 
 # ---- keys and values in pages ---------------------------------------------------------------------------------------------
 
+_INT_MAX = 0x7fffffff
 _PAGED_TYPES = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
 
 
@@ -371,7 +372,8 @@ def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, fun
     contiguous.  table (n_seq, max_pages), lens (n_seq), cu_q (n_seq + 1): int32 on the GPU.  max_q, max_len: the most queries
     / tokens of a sequence, which shape the launch (default: all rows of q, all of the table's pages).  func, block_ctx: the
     pattern (dense, block, transpose, prev); window: the query at position p sees p - window + 1 .. p (dense).  scale:
-    1 / sqrt(d_head) by default.  Returns (n_tokens, n_head, d_head); with `out`, rows outside every sequence stay as they are."""
+    1 / sqrt(d_head) by default.  Returns (n_tokens, n_head, d_head); `out` overlaps no input, and its rows outside every sequence
+    stay as they are."""
     code = _paged_type(q, kpool, vpool)
     _chk_paged(q, kpool, vpool, table, lens, cu_q, out)
     if q.dim() != 3 or kpool.dim() != 4 or kpool.shape != vpool.shape or kpool.stride() != vpool.stride() or q.shape[2] != kpool.shape[3]:
@@ -391,7 +393,7 @@ def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, fun
     a = L.AttnPagedArgs(code, func, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0) if T > 1 else H * D,
                         out.stride(1) if H > 1 else D, kpool.data_ptr(), vpool.data_ptr(), ps, rs, hs, P, page, table.data_ptr(),
                         table_stride, width, lens.data_ptr(), cu_q.data_ptr(), T, n, H, KV, D, T if max_q is None else min(max_q, T),
-                        min(width * page if max_len is None else max_len, 0x7fffffff), block_ctx or 0, window or 0,
+                        min(width * page if max_len is None else max_len, _INT_MAX), min(block_ctx or 0, _INT_MAX), min(window or 0, _INT_MAX),
                         1.0 / math.sqrt(D) if scale is None else scale, None, 0)
     lib = L.lib()
     need = lib.jb_attn_paged_workspace(C.byref(a))
@@ -442,6 +444,8 @@ def _page_pools(pools, n_pages, device):
     if len(pools) == 0:
         return L.PagePools(None, 0, n_pages, 1, 1)
     p = pools[0]
+    if p.dim() == 0:
+        raise L.JukeboxHipError("pools: expected arrays of pages")
     shape, stride, dtype, size, gpu = p.shape, p.stride(), p.dtype, p.element_size(), device.index
     n = 1
     for m, st in zip(reversed(shape[1:]), reversed(stride[1:])):
@@ -462,6 +466,8 @@ def pages_extend(table, lens, ref, cu_new, page_size, n_tokens, status):
     adds to lens, and returns the cache row of each of the n_tokens new tokens (int64; -1 behind the last).  Without enough free
     pages nothing changes, all slots are -1 and status (one int32, which the caller clears) says so."""
     t = _page_table(table, lens, ref, page_size, status)
+    if not 0 <= n_tokens <= _INT_MAX:
+        raise L.JukeboxHipError("n_tokens: expected 0 to 2^31 - 1")
     _chk_int("cu_new", cu_new, t.n_seq + 1)
     _chk_paged(table, cu_new)
     slots = torch.empty(n_tokens, dtype=torch.int64, device=table.device)
@@ -506,7 +512,7 @@ def pages_copy(pools, src, dst):
     """Page src[i] of every pool to page dst[i] (jb_pages_copy; int32 arrays).  No target twice, no target that is a source."""
     if len(pools) == 0:
         return
-    p = _page_pools(pools, pools[0].shape[0], pools[0].device)
+    p = _page_pools(pools, pools[0].shape[0] if pools[0].dim() else 0, pools[0].device)
     _chk_int("src", src)
     _chk_int("dst", dst, src.shape[0])
     _chk_paged(pools[0], src, dst)
@@ -571,7 +577,7 @@ def sample_filtered(logits, u, temp=1.0, top_k=0, top_p=0.0, min_p=0.0, out=None
             raise L.JukeboxHipError("u: expected an array with a uniform number per row")
         else:
             ptrs.append(None)
-            vals.append(x)
+            vals.append(max(min(x, _INT_MAX), 0) if name == "top_k" else x)
     _chk_paged(logits, out, *each)
     a = L.SampleFilteredArgs(code, logits.data_ptr(), logits.stride(0) if n > 1 else bins, n, bins, *ptrs, *vals[1:], out.data_ptr())
     _launch(L.lib().jb_sample_filtered, logits, C.byref(a))

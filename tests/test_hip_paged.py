@@ -288,3 +288,54 @@ def test_attention_in_a_graph_on_another_stream(H):
         b.rows_k, b.rows_v = [r[:n] for r, n in zip(b.rows_k, b.lens)], [r[:n] for r, n in zip(b.rows_v, b.lens)]
         want, tol = b.want()
         assert bool(((outs[0].double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+def test_block_and_window_as_large_as_an_int(H, dt):
+    """Blocks longer than any sequence: block is dense, prev sees nothing, transpose sees the query's own position."""
+    big = 2 ** 31 - 1
+    for nq in ([1, 1], [40, 130]):
+        b = Batch(TYPES[dt], [90, 130], nq, 4, 2, 64, 16, seed=16)
+        for func, bc, window in [(BLOCK, big, 0), (TRANSPOSE, big, 0), (DENSE, 0, big), (TRANSPOSE, big - 100, 0), (BLOCK, 2 ** 33, 0)]:
+            b.check(H, func, bc, window)
+        assert float(b.run(H, func=PREV, block_ctx=big).float().abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+@pytest.mark.parametrize("page", [5000, 4096, 65536])
+def test_one_page_holds_a_whole_sequence(H, dt, page):
+    for nq in ([1, 1], [70, 5]):
+        Batch(TYPES[dt], [3000, 41], nq, 2, 1, 64, page, seed=17, spare=0).check(H)
+
+
+def test_two_streams_at_once(H):
+    """Calls whose keys are split (each with a workspace of its own) on two streams, neither waiting for the other."""
+    a = Batch(torch.bfloat16, [4000, 900], [1, 1], 8, 2, 128, 16, seed=18)
+    c = Batch(torch.float16, [2500, 700], [60, 33], 4, 1, 64, 16, seed=19)
+    want = [a.run(H), c.run(H)]
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for stream, x, o in ((s, a, outs[0]), (t, c, outs[1])):
+            with torch.cuda.stream(stream):
+                o.append(x.run(H))
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(w, x) for x in o)
+
+
+def test_more_sequences_and_heads_than_one_launch_dimension(H):
+    """70000 sequences of a few tokens, whose workgroups are more than 65535; the last and the first are right."""
+    n, page = 70000, 4
+    g = torch.Generator("cuda").manual_seed(20)
+    k, v = (torch.randn(n, page, 1, 8, generator=g, device="cuda") for _ in range(2))
+    q = torch.randn(n, 2, 8, generator=g, device="cuda")
+    table = torch.arange(n, dtype=torch.int32, device="cuda").flip(0)[:, None].contiguous()
+    lens = torch.full((n,), 3, dtype=torch.int32, device="cuda")
+    got = H.attn_paged(q, k, v, table, lens, torch.arange(n + 1, dtype=torch.int32, device="cuda"), max_q=1)
+    kk, vv = (x.flip(0)[:, :3, 0].double() for x in (k, v))
+    s = (q.double()[:, :, None] * kk[:, None]).sum(-1) / math.sqrt(8)
+    want = (torch.softmax(s, 2)[..., None] * vv[:, None]).sum(2)
+    # scores of at most 8 products each (below 20 in all) to 8 2^-24 of theirs, the values' sum to 64 2^-24 of the largest (below 6)
+    assert float((got.double() - want).abs().max()) <= (2 * 8 * 20 + 64) * 2.0 ** -24 * 6

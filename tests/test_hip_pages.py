@@ -359,3 +359,37 @@ def test_serving_run_equals_full_attention(H):
     admit([20, 0, 0, 5, 0, 0])
     H.pages_free(table, lens, ref, ints([0, 1, 2, 3, 4, 5]), status)
     assert int(ref.abs().max()) == 0 and int(table.max()) == -1 and int(lens.max()) == 0
+
+
+def test_calls_with_nothing_to_do(H):
+    d, _ = make(H, 3, 4, 10, 16)
+    before = [x.clone() for x in (d.table, d.lens, d.ref)]
+    assert H.pages_extend(d.table, d.lens, d.ref, ints([0, 0, 0, 0]), 16, 0, d.status).numel() == 0
+    assert H.pages_extend(d.table, d.lens, d.ref, ints([0, 0, 0, 0]), 16, 5, d.status).tolist() == [-1] * 5
+    none = ints([])
+    H.pages_free(d.table, d.lens, d.ref, none, d.status)
+    H.pages_fork(d.pools, d.table, d.lens, d.ref, none, none, 16, d.status)
+    H.pages_fork([], d.table, d.lens, d.ref, ints([0]), ints([1]), 16, d.status)          # a fork of nothing: nothing
+    H.pages_copy(d.pools, none, none)
+    t2, r2 = H.pages_compact([], d.table, d.ref)
+    e = torch.empty(0, 2, 8, device="cuda", dtype=torch.float16)
+    H.kv_write(e, e, *(torch.zeros(10, 16, 2, 8, device="cuda", dtype=torch.float16) for _ in range(2)), ints([], torch.int64))
+    assert all(torch.equal(x, y) for x, y in zip(before, (d.table, d.lens, d.ref))) and int(d.status) == 0
+    assert torch.equal(t2, d.table) and torch.equal(r2, d.ref)
+    empty = ints([[0] * 4])[:0]
+    assert H.pages_extend(empty, none, d.ref, ints([0]), 16, 3, d.status).tolist() == [-1] * 3 and int(d.status) == 0
+
+
+def test_two_forks_of_one_sequence_and_ends_in_any_order(H):
+    """Both forks share the full pages (three references) and own their copies of the last; the pages come free with the last holder."""
+    page, pool = 4, torch.randn(12, 4, 5, device="cuda")
+    table, lens, ref, status = ints([[-1] * 4] * 4), ints([0] * 4), ints([0] * 12), ints([0])
+    H.pages_extend(table, lens, ref, ints([0, 0, 10, 10, 10]), page, 10, status)
+    H.pages_fork([pool], table, lens, ref, ints([1, 1]), ints([3, 0]), page, status)
+    assert ref.tolist() == [3, 3, 1, 1, 1] + [0] * 7 and lens.tolist() == [10, 10, 0, 10]
+    assert table.tolist() == [[0, 1, 4, -1], [0, 1, 2, -1], [-1] * 4, [0, 1, 3, -1]]
+    assert torch.equal(pool[3], pool[2]) and torch.equal(pool[4], pool[2])
+    H.pages_free(table, lens, ref, ints([1]), status)
+    assert ref.tolist() == [2, 2, 0, 1, 1] + [0] * 7
+    H.pages_free(table, lens, ref, ints([3, 0]), status)
+    assert int(ref.abs().max()) == 0 and int(status) == 0
