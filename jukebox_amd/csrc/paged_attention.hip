@@ -557,8 +557,9 @@ template <> struct Mfma32<f16> { static __device__ __forceinline__ f32x16 go(f16
 template <> struct Mfma32<bf16> { static __device__ __forceinline__ f32x16 go(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); } };
 
 template <int DP> struct ChunkLds {                                       // bytes
-    static constexpr int KROW = DP * 2 + 16, VROW = 64 * 2 + 16, K = 64 * KROW, V = DP * VROW, BUF = K + V;
-    static constexpr int OFF = 2 * BUF, ODD = OFF + 3 * 64 * 8, GAP = ODD + 4, ALL = GAP + 3 * 4;
+    static constexpr int KT = DP == 160 ? 32 : 64;                        // keys of a turn
+    static constexpr int KROW = DP * 2 + 16, VROW = KT * 2 + 16, K = KT * KROW, V = DP * VROW, BUF = K + V;
+    static constexpr int OFF = 2 * BUF, ODD = OFF + 3 * KT * 8, GAP = ODD + 4, ALL = GAP + 3 * 4;
 };
 __device__ __forceinline__ float swap_halves_max(float x) {              // the larger of lanes l and l ^ 32, in both
     float a = x, b = x;
@@ -567,14 +568,14 @@ __device__ __forceinline__ float swap_halves_max(float x) {              // the 
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_paged_chunk_kernel(const Args a) {
+__global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_kernel(const Args a) {
     typedef typename El<T>::vec vec;
     typedef ChunkLds<DP> L;
-    constexpr int NKS = DP / 16, NDT = DP / 32, PIECES = DP / 8, LPR = PIECES < 16 ? PIECES : 16, SETS = (PIECES + 15) / 16;
+    constexpr int KT = L::KT, NKS = DP / 16, NDT = DP / 32, PIECES = DP / 8, LPR = PIECES < 16 ? PIECES : 1024 / KT, SETS = (PIECES + LPR - 1) / LPR, OCT = KT / 8;
     constexpr int CREW = PIECES > 8 ? 2 : 1;      // waves that bring the keys' rows, and as many the values': eight pieces a lane and set
     extern __shared__ __attribute__((aligned(16))) char lds[];
     // of the turn computed, the one asked for and the one looked up:
-    int64_t* const s_off = reinterpret_cast<int64_t*>(lds + L::OFF);    // [3][64]: a key's offset in the pool, -1: nowhere
+    int64_t* const s_off = reinterpret_cast<int64_t*>(lds + L::OFF);    // [3][KT]: a key's offset in the pool, -1: nowhere
     int* const s_gap = reinterpret_cast<int*>(lds + L::GAP);            // [3]: whether a key is on no page
     int* const s_odd = reinterpret_cast<int*>(lds + L::ODD);            // whether values have been met that are no numbers
     const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
@@ -587,9 +588,9 @@ __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_paged_chunk_ker
     const T* vbase = (const T*)a.v + (int64_t)kvh * a.head_stride;
     // pieces behind the head's end are zeros throughout (the queries' are too, but 0 * NaN is not)
     if (NP < PIECES)
-        for (int i = threadIdx.x; i < 2 * 64 * (PIECES - NP); i += 256) {
+        for (int i = threadIdx.x; i < 2 * KT * (PIECES - NP); i += 256) {
             const int row = i / (PIECES - NP), pc = NP + i % (PIECES - NP);
-            *reinterpret_cast<u32x4*>(lds + (row >> 6) * L::BUF + (row & 63) * L::KROW + pc * 16) = u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(lds + row / KT * L::BUF + row % KT * L::KROW + pc * 16) = u32x4{0, 0, 0, 0};
         }
 
     for (int tile = tile0; tile < n_tiles; tile += a.tiles) {
@@ -640,13 +641,13 @@ __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_paged_chunk_ker
         __syncthreads();
         if (threadIdx.x == 0) *s_odd = 0;
         for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
-            const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n), turns = (x1 - (int)x0 + 63) / 64;
+            const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n), turns = (x1 - (int)x0 + KT - 1) / KT;
             // the first wave: where the keys of turn u are -- their pages asked for early in a turn, used at its end
-            auto page_number = [&](int u) { return (unsigned)s.table[jb_div((unsigned)(t.kb + min((int)x0 + u * 64 + lane, x1 - 1)), a.page)]; };
+            auto page_number = [&](int u) { return (unsigned)s.table[jb_div((unsigned)(t.kb + min((int)x0 + u * KT + lane % KT, x1 - 1)), a.page)]; };
             auto look_up = [&](int u, unsigned pg) {
-                const int x = (int)x0 + u * 64 + lane;
+                const int x = (int)x0 + u * KT + lane % KT;
                 const unsigned at = (unsigned)(t.kb + min(x, x1 - 1)), in_page = at - jb_div(at, a.page) * a.page.d;
-                s_off[u % 3 * 64 + lane] = x < x1 && pg < a.n_pages ? (int64_t)pg * a.page_stride + (int64_t)in_page * a.row_stride : -1;
+                s_off[u % 3 * KT + lane % KT] = x < x1 && pg < a.n_pages ? (int64_t)pg * a.page_stride + (int64_t)in_page * a.row_stride : -1;
                 const bool gap = __any(x < x1 && pg >= a.n_pages);
                 if (lane == 0) s_gap[u % 3] = gap;
             };
@@ -654,17 +655,17 @@ __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_paged_chunk_ker
             // operand.  One sequence of loads for both (a branch around them would have to wait for them at its end).
             u32x4 hold[8 * SETS];
             const bool values = wave >= CREW, works = CREW == 2 || wave < 2;
-            const int in_crew = (wave % CREW) * 64 + lane, piece = values ? (lane >> 3) + 8 * (wave % CREW) : in_crew % LPR;
-            const int key0 = values ? ((lane & 7) >> 1) * 16 + (lane & 1) * 4 : in_crew / LPR;
-            auto key_of = [&](int q) { return key0 + (values ? (q >> 2) * 8 + (q & 3) : q * 8); };
+            const int in_crew = (wave % CREW) * 64 + lane, piece = values ? lane / OCT + 64 / OCT * (wave % CREW) : in_crew % LPR;
+            const int key0 = values ? (lane % OCT >> 1) * 16 + (lane & 1) * 4 : in_crew / LPR;
+            auto key_of = [&](int q) { return key0 + (values ? (q >> 2) * 8 + (q & 3) : q * OCT); };
             auto ask = [&](int u) {               // turn u's rows into registers (of a key that is none any row will do)
-                const int64_t* off = s_off + u % 3 * 64;
+                const int64_t* off = s_off + u % 3 * KT;
                 const T* base = values ? vbase : kbase;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const T* row = base + max(off[key_of(q)], (int64_t)0);
 #pragma unroll
-                    for (int st = 0; st < SETS; ++st) hold[st * 8 + q] = load16(row + min((piece + 16 * st) * 8, D - 8));
+                    for (int st = 0; st < SETS; ++st) hold[st * 8 + q] = load16(row + min((piece + LPR * st) * 8, D - 8));
                 }
             };
             auto put = [&](int u) {               // and from there to LDS
@@ -674,15 +675,15 @@ __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_paged_chunk_ker
                     for (int q = 0; q < 8; ++q)
 #pragma unroll
                         for (int st = 0; st < SETS; ++st)
-                            if (piece + 16 * st < NP) *reinterpret_cast<u32x4*>(buf + (key0 + q * 8) * L::KROW + (piece + 16 * st) * 16) = hold[st * 8 + q];
+                            if (piece + LPR * st < NP) *reinterpret_cast<u32x4*>(buf + (key0 + q * OCT) * L::KROW + (piece + LPR * st) * 16) = hold[st * 8 + q];
                 } else {
-                    const int xb = (int)x0 + u * 64;
-                    const bool look = xb < wg_lo || xb + 64 > min(wg_hi, x1) || __builtin_amdgcn_readfirstlane(s_gap[u % 3]);
+                    const int xb = (int)x0 + u * KT;
+                    const bool look = xb < wg_lo || xb + KT > min(wg_hi, x1) || __builtin_amdgcn_readfirstlane(s_gap[u % 3]);
                     if (look) {
                         unsigned odd = 0u;
 #pragma unroll
                         for (int q = 0; q < 8; ++q) {
-                            const bool none = s_off[u % 3 * 64 + key_of(q)] < 0;
+                            const bool none = s_off[u % 3 * KT + key_of(q)] < 0;
 #pragma unroll
                             for (int st = 0; st < SETS; ++st)
 #pragma unroll
@@ -696,9 +697,9 @@ __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_paged_chunk_ker
                     }
 #pragma unroll
                     for (int st = 0; st < SETS; ++st)
-                        if (piece + 16 * st < PIECES) {
+                        if (piece + LPR * st < PIECES) {
                             const u32x4 w[8] = {hold[st * 8], hold[st * 8 + 1], hold[st * 8 + 2], hold[st * 8 + 3], hold[st * 8 + 4], hold[st * 8 + 5], hold[st * 8 + 6], hold[st * 8 + 7]};
-                            char* at = buf + L::K + (piece + 16 * st) * 8 * L::VROW + (lane & 7) * 16;
+                            char* at = buf + L::K + (piece + LPR * st) * 8 * L::VROW + lane % OCT * 16;
 #pragma unroll
                             for (int e = 0; e < 8; ++e) *reinterpret_cast<u32x4*>(at + e * L::VROW) = __builtin_bit_cast(u32x4, gather(w, e, f16()));
                         }
@@ -716,11 +717,11 @@ __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_paged_chunk_ker
                 if (works) ask(min(u + 1, turns - 1));
                 const unsigned pg = page_number(u + 2);
                 const char* buf = lds + (u & 1) * L::BUF;
-                const int64_t* off = s_off + u % 3 * 64 + h * 4;
+                const int64_t* off = s_off + u % 3 * KT + h * 4;
                 const bool gap = __builtin_amdgcn_readfirstlane(s_gap[u % 3]);
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub) {
-                    const int xb = (int)x0 + u * 64 + sub * 32;
+                for (int sub = 0; sub < KT / 32; ++sub) {
+                    const int xb = (int)x0 + u * KT + sub * 32;
                     if (xb >= min(any_hi, x1) || xb + 32 <= any_lo) continue;         // none of the wave's rows sees any of them
                     f32x16 sc;
 #pragma unroll
@@ -778,8 +779,8 @@ __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void attn_paged_chunk_ker
             for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
                 const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n);
                 for (int x = (int)x0; x < x1; ++x) {
-                    const int xb = (int)x0 + (x - (int)x0) / 64 * 64;
-                    if (xb >= wg_lo && xb + 64 <= min(wg_hi, x1)) continue;
+                    const int xb = (int)x0 + (x - (int)x0) / KT * KT;
+                    if (xb >= wg_lo && xb + KT <= min(wg_hi, x1)) continue;
                     const unsigned row = __builtin_amdgcn_readfirstlane(cache_row(a, s, t.kb + x));
                     if (row == BAD) continue;
                     const T *vp = vbase + cache_offset(a, row), *kp = kbase + cache_offset(a, row);
