@@ -541,14 +541,16 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
 // Chunks: one workgroup of four waves per (sequence, kv head, tile of 128 rows, split of the keys), a wave 32 rows.
 //
 // The same two products on 32 x 32 x 16 matrix instructions: S^T = K Q^T leaves a lane the scores of 16 of 32 keys for row l & 31, which
-// are the B operand of O^T += V^T P^T once slot (h, i) of a k-step s is key 16 s + 8 (i / 4) + 4 h + i % 4.  64 keys at a time go through LDS,
+// are the B operand of O^T += V^T P^T once slot (h, i) of a k-step s is key 16 s + 8 (i / 4) + 4 h + i % 4.  64 keys at a time go through LDS
+// (32 under heads of 129-160 channels, so that two workgroups of them fit a compute unit: 4 x 2048 queries 652 us against 858),
 // two buffers, one barrier a turn: half the waves bring the keys' rows, the others the values', transposed on the way by byte
 // permutations ([channel][key], so that an operand is one 16-byte read), all asked for a turn ahead.  LDS rows are padded by 16 bytes: the
 // 16 lanes of a read phase then hit 16 different groups of four banks.
 // The probabilities enter the second product rounded once to 16 bits, which adds an error of the size of the output's own
 // rounding (each is off by half a step, and they average); a second product for the rest would cost a quarter of the rate.
 // Measured (32 heads on 8 of 128 channels, bf16, pages of 64; the library's product of 16384^3 runs at 1370 TFLOP/s): 4 x 2048 queries behind
-// 6144 keys: 1.22 ms, 790 TFLOP/s; 4 x 257-2048 behind 4097-8192: 745 us, 635 TFLOP/s.  Two workgroups share a compute unit, and the
+// 6144 keys: 1.22 ms, 790 TFLOP/s; 4 x 257-2048 behind 4097-8192: 670-750 us from card to card, 630-700
+// TFLOP/s; 8 heads of 150, f16, 100-1000 queries behind 1000-5000: 120 us, 244 TFLOP/s.  Two workgroups share a compute unit, and the
 // products' 27 % of the time hide behind the softmax's exponentials and the LDS reads, of which either alone would take about as long
 // as the products at their peak.  Waves of 64 rows, which halve the LDS reads but leave one wave a SIMD (and its registers spilling): 1.13 ms
 // instead of 0.83 for the second case as things then were.
@@ -913,10 +915,12 @@ Plan plan_of(const jb_attn_paged_args* p) {
         if (chunk > 2048) chunk = 2048;
         if (chunk < 256) chunk = wgs * w.range <= 64 * 256 ? 64 : 256;
     }
-    // chunks: their turns are long enough from 512 keys on (24 tiles that hold rows, 5000 keys: 149 us; unsplit 236; aimed at 512 or 2048
-    // workgroups instead of 1024: 165, 185)
-    if (w.tr > 16 && wgs < 1024 && w.range > 512) {
-        chunk = (wgs * w.range / 1024 + 127) / 128 * 128;
+    // Chunks: two workgroups a compute unit as well, by the tiles that there can be in all (sequences are rarely as long as the longest:
+    // 3 of 100-1000 queries, 5000 keys under 8 heads of 150: 120 us, split for as many tiles as the launch has 168; 1000 queries of one
+    // sequence: 80 us; three or four workgroups a unit: 103; one and a half: 95), and 512 keys at least.
+    const int64_t filled = (p->n_tokens * G + w.tr - 1) / w.tr + p->n_seq / 2, real = filled * p->n_kv_head < wgs ? filled * p->n_kv_head : wgs;
+    if (w.tr > 16 && real < 1024 && w.range > 512) {
+        chunk = (real * w.range / 512 + 127) / 128 * 128;
         if (chunk < 512) chunk = 512;
     }
     if (chunk) {
