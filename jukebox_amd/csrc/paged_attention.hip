@@ -846,11 +846,12 @@ __global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_ker
 // Joins the splits' states of rows that were split: a wave 64 channels of a row of a tile, four a lane, a quarter of the splits each
 // sixteen lanes; their weights one a lane.  (A wave a row left 16 waves to read 32 states of 480 channels: 19 us, now 5.)
 template <typename T>
-__global__ __launch_bounds__(64) void attn_paged_join_kernel(const Args a, int tile_rows) {
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(const Args a, int tile_rows) {
     int64_t b = blockIdx.x;
-    const int wr = (int)(b % tile_rows); b /= tile_rows;
+    const int fours = (tile_rows + 3) / 4, wr = (int)(b % fours) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); b /= fours;
+    if (wr >= tile_rows) return;
     const int tile0 = (int)(b % a.tiles); b /= a.tiles;
-    const int kvh = (int)(b % a.n_kv), si = (int)(b / a.n_kv), lane = threadIdx.x, part_of = lane >> 4;
+    const int kvh = (int)(b % a.n_kv), si = (int)(b / a.n_kv), lane = threadIdx.x & 63, part_of = lane >> 4;
     const Seq s = seq_of(a, si);
     const int n_tiles = tiles_of(a, s.nq), d0 = blockIdx.y * 64 + (lane & 15) * 4, d = min(d0, a.D - 4);     // (a last piece begins four before the end)
     for (int tile = tile0; tile < n_tiles; tile += a.tiles) {
@@ -924,7 +925,9 @@ Plan plan_of(const jb_attn_paged_args* p) {
         if (chunk < 512) chunk = 512;
     }
     if (chunk) {
-        if ((w.range + chunk - 1) / chunk > 64) chunk = ((w.range + 63) / 64 + 127) / 128 * 128;      // the join holds 64 states
+        // the join holds 64 states; a batch padded far beyond its sequences' rows gets fewer, so that 1 GiB holds them
+        const int64_t fit = (1ll << 30) / ((int64_t)p->n_tokens * p->n_head * (p->d_head + 2) * 4), most = fit < 1 ? 1 : fit < 64 ? fit : 64;
+        if ((w.range + chunk - 1) / chunk > most) chunk = ((w.range + most - 1) / most + 127) / 128 * 128;
         if (w.range > chunk) { w.splits = (int)((w.range + chunk - 1) / chunk); w.chunk = (unsigned)chunk; }
     }
     return w;
@@ -1024,7 +1027,10 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     }
     hipStream_t s = (hipStream_t)stream;
     const int64_t most_rows = (int64_t)a->max_q * k.G;
-    const int tile_rows = (int)(most_rows < 16 ? most_rows : 16);
+    // waves that join a tile: 16, each several rows of a chunk one after the other (24 tiles under 8 heads, 5 states: 22 us; more waves, whose
+    // beginnings cost as much as a row, 45) -- more where tiles are so few that the waves find room at once (8 tiles, 59 states: 61 -> 50 in all)
+    const int64_t room = wgs < 64 ? 1024 / wgs : 16, side = w.tr == 16 ? 16 : room < 128 ? room : 128;
+    const int tile_rows = (int)(most_rows < side ? most_rows : side);
     JB_REQUIRE(w.splits == 1 || wgs * tile_rows <= 0x7fffffff, "grid too large");
 #define JB_ROWS(T, CH)                                                            \
     do {                                                                          \
@@ -1033,7 +1039,7 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
         else if (a->d_head <= 256) launch_rows<T, 256 / CH>(k, grid, s);          \
         else launch_rows<T, 512 / CH>(k, grid, s);                                \
         JB_CHECK_LAUNCH();                                                        \
-        if (w.splits > 1) attn_paged_join_kernel<T><<<dim3((unsigned)(wgs * tile_rows), (unsigned)((a->d_head + 63) / 64)), 64, 0, s>>>(k, tile_rows); \
+        if (w.splits > 1) attn_paged_join_kernel<T><<<dim3((unsigned)(wgs * ((tile_rows + 3) / 4)), (unsigned)((a->d_head + 63) / 64)), 256, 0, s>>>(k, tile_rows); \
     } while (0)
     if (a->dtype == JB_F16) JB_ROWS(f16, 128);
     else if (a->dtype == JB_BF16) JB_ROWS(bf16, 128);

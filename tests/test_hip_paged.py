@@ -339,3 +339,14 @@ def test_more_sequences_and_heads_than_one_launch_dimension(H):
     want = (torch.softmax(s, 2)[..., None] * vv[:, None]).sum(2)
     # scores of at most 8 products each (below 20 in all) to 8 2^-24 of theirs, the values' sum to 64 2^-24 of the largest (below 6)
     assert float((got.double() - want).abs().max()) <= (2 * 8 * 20 + 64) * 2.0 ** -24 * 6
+
+
+def test_a_batch_padded_far_beyond_its_rows(H):
+    """A buffer of 300000 rows of which five are queries: split as far as a workspace of 1 GiB allows."""
+    b = Batch(torch.bfloat16, [6000, 900], [3, 2], 8, 2, 64, 16, seed=21)
+    q = torch.full((300000, 8, 64), math.nan, device="cuda", dtype=torch.bfloat16)
+    q[:5] = b.q
+    out = torch.full_like(q, 7.0)
+    H.attn_paged(q, b.k, b.v, b.table, b.len_t, b.cu, max_q=3, out=out)
+    want, tol = b.want()
+    assert bool(((out[:5].double() - want).abs() <= tol).all()) and bool((out[5:] == 7.0).all())

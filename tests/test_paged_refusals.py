@@ -163,3 +163,12 @@ def test_python_layer_refuses_wrong_tensors(lib):
         with pytest.raises(JukeboxHipError):
             call()
     assert H.pages_copy([], i(0), i(0)) is None
+
+
+@pytest.mark.parametrize("n_tokens,max_q,d_head", [(65536, 1, 128), (65536, 1, 512), (400000, 1, 64), (1 << 22, 4, 128), (65536, 300, 128)])
+def test_workspace_of_a_padded_batch(lib, n_tokens, max_q, d_head):
+    """Four sequences in buffers of many more rows: the split states take 1 GiB at most."""
+    need = lib.jb_attn_paged_workspace(C.byref(attn(n_tokens=n_tokens, n_seq=4, n_head=32, n_kv_head=8, d_head=d_head, q_row_stride=32 * d_head,
+                                                    out_row_stride=32 * d_head, q_head_stride=d_head, out_head_stride=d_head, max_q=max_q,
+                                                    max_len=131072, max_pages=8192)))
+    assert 0 <= need <= 1 << 30
