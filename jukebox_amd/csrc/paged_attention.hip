@@ -845,7 +845,8 @@ __global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_ker
 
 // Joins the splits' states of rows that were split: a wave 64 channels of a row of a tile, four a lane, a quarter of the splits each
 // sixteen lanes; their weights one a lane.  (A wave a row left 16 waves to read 32 states of 480 channels: 19 us, now 5.)
-template <typename T>
+// U: fours of splits at most; ROWS: rows whose states are asked for together (four: the 150-channel chunks 120 -> 116 us in all).
+template <typename T, int U, int ROWS>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(const Args a, int tile_rows) {
     int64_t b = blockIdx.x;
     const int fours = (tile_rows + 3) / 4, wr = (int)(b % fours) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); b /= fours;
@@ -858,32 +859,42 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(const Args a, int 
         const Tile t = tile_of(a, s, tile);
         const int n_act = active_splits(a, t.n);
         if (n_act < 2) continue;
-        for (int R = t.row0 + wr; R < min(t.row0 + a.tr, t.rows); R += tile_rows) {
-            const int i = (int)jb_div(R, a.group);
-            const int64_t tok = s.t0 + t.j0 + i * t.js;
-            const int h = kvh * a.G + (R - i * a.G);
-            const float* ml = a.ml + (tok * a.n_head + h) * a.splits * 2;
-            const float* part = a.part + (tok * a.n_head + h) * a.splits * (int64_t)a.D + d;
-            const float m = lane < n_act ? ml[2 * lane] : -INFINITY, l = lane < n_act ? ml[2 * lane + 1] : 0.f;      // at most 64 splits
-            f32x4 v[16];
+        const int end = min(t.row0 + a.tr, t.rows);
+        for (int R0 = t.row0 + wr; R0 < end; R0 += tile_rows * ROWS) {
+            f32x4 v[ROWS][U];
+            float m[ROWS], l[ROWS];
+            int64_t to[ROWS];
 #pragma unroll
-            for (int u = 0; u < 16; ++u)
-                if (u * 4 < n_act) v[u] = __builtin_bit_cast(f32x4, *reinterpret_cast<const u32x4_any*>(part + (int64_t)min(u * 4 + part_of, n_act - 1) * a.D));
-            const float M = jb_wave_max(m), base = M == -INFINITY ? 0.f : M, e = __builtin_amdgcn_exp2f(m - base), L = jb_wave_sum(l * e);
-            const float w = L != 0.f ? e / L : 0.f;
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+            for (int r = 0; r < ROWS; ++r) {
+                const int R = min(R0 + r * tile_rows, end - 1), i = (int)jb_div(R, a.group), h = kvh * a.G + (R - i * a.G);
+                const int64_t tok = s.t0 + t.j0 + i * t.js, state = (tok * a.n_head + h) * a.splits;
+                const float *ml = a.ml + state * 2, *part = a.part + state * (int64_t)a.D + d;
+                to[r] = tok * a.o_row + (int64_t)h * a.o_head + d;
+                m[r] = lane < n_act ? ml[2 * lane] : -INFINITY;
+                l[r] = lane < n_act ? ml[2 * lane + 1] : 0.f;
 #pragma unroll
-            for (int u = 0; u < 16; ++u)
-                if (u * 4 < n_act) {
-                    const float wu = __shfl(w, u * 4 + part_of);          // (a lane behind the last split weighs nothing)
-                    o += v[u] * wu;
+                for (int u = 0; u < U; ++u)
+                    if (u * 4 < n_act) v[r][u] = __builtin_bit_cast(f32x4, *reinterpret_cast<const u32x4_any*>(part + (int64_t)min(u * 4 + part_of, n_act - 1) * a.D));
+            }
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                if (R0 + r * tile_rows >= end) break;
+                const float M = jb_wave_max(m[r]), base = M == -INFINITY ? 0.f : M, e = __builtin_amdgcn_exp2f(m[r] - base), L = jb_wave_sum(l[r] * e);
+                const float w = L != 0.f ? e / L : 0.f;
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (u * 4 < n_act) {
+                        const float wu = __shfl(w, u * 4 + part_of);      // (a lane behind the last split weighs nothing)
+                        o += v[r][u] * wu;
+                    }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = jb_rows_reduce(o[k], [](float x, float y) { return x + y; });
+                if (part_of == 0 && d0 < a.D) {
+                    T* q = (T*)a.out + to[r];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) q[k] = (T)o[k];
                 }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = jb_rows_reduce(o[k], [](float x, float y) { return x + y; });
-            if (part_of == 0 && d0 < a.D) {
-                T* q = (T*)a.out + tok * a.o_row + (int64_t)h * a.o_head + d;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) q[k] = (T)o[k];
             }
         }
     }
@@ -1027,8 +1038,8 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     }
     hipStream_t s = (hipStream_t)stream;
     const int64_t most_rows = (int64_t)a->max_q * k.G;
-    // waves that join a tile: 16, each several rows of a chunk one after the other (24 tiles under 8 heads, 5 states: 22 us; more waves, whose
-    // beginnings cost as much as a row, 45) -- more where tiles are so few that the waves find room at once (8 tiles, 59 states: 61 -> 50 in all)
+    // waves that join a tile: 16, each several rows of a chunk (24 tiles under 8 heads, 5 states: 122 us in all; 64 waves, whose beginnings cost
+    // as much as a row, 131) -- more where tiles are so few that the waves find room at once (8 tiles, 59 states: 61 -> 51)
     const int64_t room = wgs < 64 ? 1024 / wgs : 16, side = w.tr == 16 ? 16 : room < 128 ? room : 128;
     const int tile_rows = (int)(most_rows < side ? most_rows : side);
     JB_REQUIRE(w.splits == 1 || wgs * tile_rows <= 0x7fffffff, "grid too large");
@@ -1039,7 +1050,11 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
         else if (a->d_head <= 256) launch_rows<T, 256 / CH>(k, grid, s);          \
         else launch_rows<T, 512 / CH>(k, grid, s);                                \
         JB_CHECK_LAUNCH();                                                        \
-        if (w.splits > 1) attn_paged_join_kernel<T><<<dim3((unsigned)(wgs * ((tile_rows + 3) / 4)), (unsigned)((a->d_head + 63) / 64)), 256, 0, s>>>(k, tile_rows); \
+        if (w.splits > 1) {                                                       \
+            const dim3 g((unsigned)(wgs * ((tile_rows + 3) / 4)), (unsigned)((a->d_head + 63) / 64)); \
+            if (w.splits <= 16) attn_paged_join_kernel<T, 4, 4><<<g, 256, 0, s>>>(k, tile_rows); \
+            else attn_paged_join_kernel<T, 16, 1><<<g, 256, 0, s>>>(k, tile_rows); \
+        }                                                                         \
     } while (0)
     if (a->dtype == JB_F16) JB_ROWS(f16, 128);
     else if (a->dtype == JB_BF16) JB_ROWS(bf16, 128);
