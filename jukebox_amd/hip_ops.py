@@ -1,7 +1,8 @@
 """Thin tensor-level wrappers over the C ABI (include/jukebox_hip.h).
 
 torch supplies device memory and the current HIP stream only; every computation below happens
-in libjukebox_hip.so.  Tensors must live on the GPU and be contiguous; there is no CPU path.
+in libjukebox_hip.so.  Tensors must live on the GPU and be contiguous unless a function says
+otherwise; there is no CPU path.
 """
 import ctypes as C
 import math
