@@ -327,8 +327,10 @@ int jb_vq_argmin(const float* x, const float* xk, const float* codebook, int64_t
  * nor written; out overlaps no input.  n_head / n_kv_head consecutive query heads share a key / value head.  A query without a visible key (block 0
  * of the prev pattern, a length below the number of queries) gives zeros; a masked key or value may hold anything, NaN too;
  * positions whose table entry is no page number are masked.  Patterns 0-3; `window` (dense only, 0 = off): the query at p sees
- * positions p - window + 1 .. p.  Strides in elements, channels contiguous; k and v share them.  Softmax in fp32; 16-bit
- * outputs are rounded once. */
+ * positions p - window + 1 .. p.  Strides in elements, channels contiguous; k and v share them.  Scores, softmax and sums in fp32;
+ * 16-bit outputs are rounded once.  In 16 bits a probability enters the value product as the sum of two numbers of the type (off by
+ * 2^-16 of itself in bf16, 2^-22 in f16) -- but rounded to one (2^-8, 2^-11) in the kernel of chunks, which takes calls of heads of up
+ * to 256 channels, not the transpose pattern, with max_q * (n_head / n_kv_head) >= 64. */
 typedef struct jb_attn_paged_args {
     int dtype, attn_func;                              /* JB_F32, JB_F16, JB_BF16; of q, k, v and out */
     const void* q; int64_t q_row_stride, q_head_stride;

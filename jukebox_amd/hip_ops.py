@@ -374,7 +374,10 @@ def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, fun
     / tokens of a sequence, which shape the launch (default: all rows of q, all of the table's pages).  func, block_ctx: the
     pattern (dense, block, transpose, prev); window: the query at position p sees p - window + 1 .. p (dense).  scale:
     1 / sqrt(d_head) by default.  Returns (n_tokens, n_head, d_head); `out` overlaps no input, and its rows outside every sequence
-    stay as they are."""
+    stay as they are.
+
+    In 16 bits, calls with max_q * n_head / n_kv_head >= 64, heads of up to 256 channels and no transpose pattern go to the kernel of
+    chunks, which rounds the probabilities to the type once; all others carry them in two parts (jb_attn_paged has the bounds)."""
     code = _paged_type(q, kpool, vpool)
     _chk_paged(q, kpool, vpool, table, lens, cu_q, out)
     if q.dim() != 3 or kpool.dim() != 4 or kpool.shape != vpool.shape or kpool.stride() != vpool.stride() or q.shape[2] != kpool.shape[3]:

@@ -1,0 +1,99 @@
+"""GPU suite: the paged attention where its inputs are at their limits -- probabilities far below the largest, infinite keys and values that
+are seen, table entries that name no page inside a chunk, sizes at the end of what a call may have -- against 64 bits.
+
+The tolerance is test_hip_paged.py's, with the probabilities' own term by the kernel that the call takes:
+    |got - want| <= u |want| + (2 ds + dp + n 2^-24) sum_k p_k |v_k| + 2^-39 sum_k |v_k| (half) + half a step of the smallest half
+  dp  2^-16 (bfloat16), 2^-22 (half) where the probabilities enter in two parts; 2^-8, 2^-11 in the kernel of chunks (heads of up to 256
+      channels, not the transpose pattern, 64 rows and more: max_q * heads / kv); plus 2^-22 for the exponential
+  2^-39  halfs below 2^-14 have an absolute step of 2^-24: half of it, of probabilities that enter 2^14 times as large
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_hip_paged import DENSE, TRANSPOSE, TYPES, Batch, visible  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def H():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from jukebox_amd import _lib, hip_ops
+    _lib.lib()          # fail loudly if the extension is missing
+    return hip_ops
+
+
+class Made(Batch):
+    """A batch whose rows are given: keys(i), values(i) of sequence i as (len, kv, D), queries as (rows, heads, D)."""
+
+    def __init__(self, dtype, lens, nq, heads, kv, D, page, keys=None, values=None, queries=None, **kw):
+        super().__init__(dtype, lens, nq, heads, kv, D, page, **kw)
+        for i, n in enumerate(lens):
+            pos = torch.arange(n, device="cuda")
+            pg = self.table[i, pos // page].long()
+            for made, pool, rows in ((keys, self.k, self.rows_k), (values, self.v, self.rows_v)):
+                if made is not None:
+                    x = made(i).to(dtype)
+                    pool[pg, pos % page] = x
+                    rows[i] = x.double()
+        if queries is not None:
+            self.q = queries.to(dtype)
+
+    def chunks(self, func, max_q=None):
+        """Whether the call takes the kernel of chunks."""
+        rows = (sum(self.nq) if max_q is None else max_q) * self.heads // self.kv
+        return self.dtype != torch.float32 and func != TRANSPOSE and self.D <= 256 and rows >= 64
+
+    def fine(self, func=DENSE, bc=0, window=0, max_q=None):
+        """(values, tolerances) in 64 bits."""
+        scale, u, at = 1.0 / math.sqrt(self.D), torch.finfo(self.dtype).eps / 2, 0
+        half, two = self.dtype == torch.float16, not self.chunks(func, max_q)
+        dp = {torch.float32: 0.0, torch.float16: 2.0 ** (-22 if two else -11), torch.bfloat16: 2.0 ** (-16 if two else -8)}[self.dtype] + 2.0 ** -22
+        out = torch.zeros(self.q.shape, dtype=torch.float64, device="cuda")
+        tol = torch.full_like(out, 1e-30)
+        for i, (n, nq) in enumerate(zip(self.lens, self.nq)):
+            q = self.q[at:at + nq].double()
+            see = visible(func, bc, window, torch.arange(n - nq, n, device="cuda")[:, None], torch.arange(n, device="cuda")[None, :])
+            for h in range(self.heads):
+                k, v = (r[i][:, h * self.kv // self.heads] for r in (self.rows_k, self.rows_v))
+                s = torch.where(see, (q[:, h] @ k.T) * scale, -math.inf)
+                ds = self.D * 2.0 ** -24 * (q[:, h].abs() @ k.abs().T) * scale + 3 * 2.0 ** -24 * torch.where(see, s.abs(), 0.0)
+                p = torch.softmax(s, 1)
+                o = p @ v
+                # a score's error moves its own probability, and all of them through the sum
+                mean = (p * ds).sum(1, keepdim=True)
+                out[at:at + nq, h] = o
+                tol[at:at + nq, h] += (u * o.abs() + (1 + u) * ((p * ds) @ v.abs() + (mean + dp + (n / 64 + 64) * 2.0 ** -24) * (p @ v.abs()))
+                                       + (2.0 ** -39 * (see.double() @ v.abs()) + 2.0 ** -25 if half else 0.0))
+            at += nq
+        return out, tol
+
+    def check_fine(self, H, **kw):
+        got = self.run(H, **{{"bc": "block_ctx"}.get(k, k): v for k, v in kw.items()})
+        torch.cuda.synchronize()
+        want, tol = self.fine(**kw)
+        off = (got.double() - want).abs()
+        assert bool((off <= tol).all()), f"off by {float((off / tol).max()):.3g} tolerances, {int((~(off <= tol)).sum())} of {off.numel()} elements"
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("heads,kv,D,lens,nq,kw", [
+    (2, 2, 64, [5, 7], [1, 1], {}), (4, 2, 128, [6], [2], {}), (1, 1, 250, [5], [3], {}), (1, 1, 480, [7], [2], {}), (3, 3, 300, [40], [34], {"window": 5}),
+    (2, 1, 40, [90], [80], {"func": TRANSPOSE, "bc": 20}), (1, 1, 480, [100], [90], {"window": 6}), (2, 1, 64, [100], [70], {"window": 5})],
+    ids=["one", "two", "250", "480", "300", "transpose", "chunk480", "chunk64"])
+def test_values_that_cancel(H, dt, page, heads, kv, D, lens, nq, kw):
+    """Neighbouring values of opposite signs, so that an output is far below what its products add up to and the probabilities' own
+    rounding shows.  Few keys a query, short queries: the scores' error is below it."""
+    g = torch.Generator("cuda").manual_seed(D)
+
+    def values(i):
+        n = lens[i]
+        sign = 1.0 - 2.0 * (torch.arange(n, device="cuda") // (20 if kw.get("func") == TRANSPOSE else 1) % 2)
+        return sign[:, None, None] * (1 + 0.01 * torch.randn(n, kv, D, generator=g, device="cuda"))
+
+    q = 0.5 / math.sqrt(D) * torch.randn(sum(nq), heads, D, generator=g, device="cuda")
+    Made(TYPES[dt], lens, nq, heads, kv, D, page, values=values, queries=q, seed=D).check_fine(H, **kw)
