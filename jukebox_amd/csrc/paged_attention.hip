@@ -14,20 +14,29 @@ template <> struct El<f16> {
     typedef f16x8 vec;
     static constexpr int E = 8;
     static constexpr unsigned ABS = 0x7fff7fffu, STEP = 0x04000400u;      // of two elements: without the sign; the exponent's lowest bit
+    static constexpr float LIFT = 14.f;                                   // see reference_of
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct El<bf16> {
     typedef bf16x8 vec;
     static constexpr int E = 8;
     static constexpr unsigned ABS = 0x7fff7fffu, STEP = 0x00800080u;
+    static constexpr float LIFT = 0.f;
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct El<float> {
     typedef f32x4 vec;
     static constexpr int E = 4;
     static constexpr unsigned ABS = 0x7fffffffu, STEP = 0x00800000u;
+    static constexpr float LIFT = 0.f;
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return jb_mfma(a, b, c); }
 };
+
+// A row's probabilities are 2^(score - m) with m the running maximum less LIFT (scores in units of log2 e).  A half is subnormal below
+// 2^-14 and 0 below 2^-25: unlifted, the 8000 keys 18 nats below one other were lost from the values' sum and not from the weights'.  Up to
+// 2^14 = a quarter of the largest half they keep their bits down to 2^-28 of the largest.  (What m is exactly does not matter, as a state's
+// sum, values and m go together -- but that no probability passes 2^15: far scores, of which 14 is within a rounding or two, go unlifted.)
+template <typename T> __device__ __forceinline__ float reference_of(float mx) { return El<T>::LIFT != 0.f && fabsf(mx) < 0x1p20f ? mx - El<T>::LIFT : mx; }
 
 struct Args {
     const void* q; int64_t q_row, q_head;
@@ -163,8 +172,8 @@ template <typename T> __device__ __forceinline__ void store8(T* o, const float* 
 //   O^T += V^T P^T  the order of a product's inner index is free: slot (g, i) is key (i / 4) * 16 + g * 4 + i % 4, so the B
 //                   operand is the lane's own probabilities, and the A operand the lane's own eight value pieces (gather above).
 // K and V therefore go from memory to the matrix cores through registers alone.
-// In 16 bits the probabilities enter as a high and a low part (two products): the output is as near the 64-bit value as its own
-// rounding allows; the products hide behind the memory anyway (one new token: 1 row of 16 used).
+// In 16 bits the probabilities enter as a high and a low part (two products), off by 2^-16 of themselves in bf16 and 2^-22 in f16 (those
+// above 2^-28 of the largest, see reference_of; an absolute 2^-39 below): the output is as near the 64-bit value as its own rounding allows; the products hide behind the memory anyway (one new token: 1 row of 16 used).
 // NC slices of 16 E channels cover d_head, each a wave's: heads of up to 128 halfs have four waves side by side on the keys, every
 // one with a running maximum and sum of its own, joined through LDS at the end; wider heads NC waves to a turn of 32 keys, which add
 // up their parts of the scores through LDS (one barrier a turn).  One wave for a whole head of 480 channels held 512 registers, four
@@ -248,7 +257,7 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
         f32x4 acc[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m = -INFINITY, l = 0.f;            // of the lane's row: the maximum the same in its four lanes, the sum a part in each
+        float m = -INFINITY, l = 0.f;            // of the lane's row: the reference the same in its four lanes, the sum a part in each
 
         // One turn: the scores' parts so far in sc, the values in vf.  gone: bit i, no page holds key i.
         auto turn = [&](f32x4 (&sc)[2], u32x4 (&vf)[8], int xb, int x1, unsigned gone, auto value_row) {
@@ -270,7 +279,7 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
 #pragma unroll
             for (int i = 0; i < 8; ++i) mx = fmaxf(mx, p[i]);
             mx = jb_rows_reduce(mx, [](float u, float v) { return fmaxf(u, v); });
-            const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.f : m_new;
+            const float m_new = fmaxf(m, reference_of<T>(mx)), base = m_new == -INFINITY ? 0.f : m_new;
             if (__any(m_new != m)) {
                 const float alpha = __builtin_amdgcn_exp2f(m - base);
                 l *= alpha;
@@ -634,7 +643,7 @@ __global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_ker
         walk(pos_of(min(t.row0 + a.tr, t.rows) - 1), wg_lo, unused);
 
         f32x16 acc[NDT];
-        float m = -INFINITY, l = 0.f;            // of the lane's row: the maximum the same in both its lanes, the sum a part in each
+        float m = -INFINITY, l = 0.f;            // of the lane's row: the reference the same in both its lanes, the sum a part in each
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -745,7 +754,7 @@ __global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_ker
                     float mx = -INFINITY;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[r]);
-                    const float m_new = fmaxf(m, swap_halves_max(mx) * a.c_abs), base = m_new == -INFINITY ? 0.f : m_new;
+                    const float m_new = fmaxf(m, reference_of<T>(swap_halves_max(mx) * a.c_abs)), base = m_new == -INFINITY ? 0.f : m_new;
                     if (__any(m_new != m)) {
                         const float alpha = __builtin_amdgcn_exp2f(m - base);
                         l *= alpha;

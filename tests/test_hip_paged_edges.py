@@ -97,3 +97,60 @@ def test_values_that_cancel(H, dt, page, heads, kv, D, lens, nq, kw):
 
     q = 0.5 / math.sqrt(D) * torch.randn(sum(nq), heads, D, generator=g, device="cuda")
     Made(TYPES[dt], lens, nq, heads, kv, D, page, values=values, queries=q, seed=D).check_fine(H, **kw)
+
+
+def peaked(dt, heads, kv, D, lens, nq, page, nats, seed):
+    """The first key of every sequence `nats` above thousands of others; its value 0, the others' 1."""
+    g = torch.Generator("cuda").manual_seed(seed)
+
+    def keys(i):
+        k = 0.01 * torch.randn(lens[i], kv, D, generator=g, device="cuda")
+        k[:, :, 0] = -nats
+        k[0, :, 0] = 0.0
+        return k
+
+    def values(i):
+        v = torch.ones(lens[i], kv, D, device="cuda")
+        v[0] = 0.0
+        return v
+
+    q = 0.1 * torch.randn(sum(nq), heads, D, generator=g, device="cuda")
+    q[:, :, 0] = math.sqrt(D)
+    return Made(TYPES[dt], lens, nq, heads, kv, D, page, keys=keys, values=values, queries=q, seed=seed)
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+@pytest.mark.parametrize("nats", [8.0, 14.0, 17.0, 17.5, 18.0, 20.0, 24.0])
+@pytest.mark.parametrize("heads,kv,D,lens,nq,page", [
+    (2, 2, 64, [8000], [1], 16), (2, 1, 128, [5000, 3001], [2, 1], 7), (1, 1, 480, [4096], [1], 64), (1, 1, 256, [4096, 77], [3, 1], 16),
+    (1, 1, 64, [8000], [80], 16), (4, 2, 128, [3000, 600], [200, 40], 20), (2, 2, 150, [2500], [130], 32), (1, 1, 256, [3000], [70], 16), (8, 8, 64, [2000] * 40, [1] * 40, 16)],
+    ids=["one", "few", "480", "256", "chunk64", "chunk128", "chunk150", "chunk256", "batch"])
+def test_one_key_far_above_thousands(H, dt, nats, heads, kv, D, lens, nq, page):
+    """An attention sink: the long tail's share, far below 2^-14, carries the whole output."""
+    peaked(dt, heads, kv, D, lens, nq, page, nats, seed=D).check_fine(H)
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+@pytest.mark.parametrize("nq", [1, 80])
+@pytest.mark.parametrize("size", [40.0, 1000.0])
+def test_scores_far_from_zero(H, dt, nq, size):
+    """Scores of 10^4 and 10^7, up and down: one key takes all, the others nothing, and no probability passes the type's range."""
+    for D in (64, 480):
+        for sign in (1.0, -1.0):
+            n = 200
+            step = torch.arange(n, device="cuda").double() / n
+
+            def keys(i):
+                k = torch.zeros(n, 1, D, device="cuda")
+                k[:, 0, :] = (sign * size * (1 + step))[:, None]
+                return k
+
+            b = Made(TYPES[dt], [n], [nq], 1, 1, D, 16, keys=keys, queries=torch.full((nq, 1, D), size, device="cuda"), seed=5)
+            got = b.run(H).double()
+            s = (b.q[:, 0].double() @ b.rows_k[0][:, 0].T) / math.sqrt(D)
+            for r in range(nq):
+                seen = n - nq + r + 1
+                # (rows of one rounded value tie exactly; they share)
+                p = torch.softmax(s[r, :seen], 0)
+                want = p @ b.rows_v[0][:seen, 0]
+                assert float((got[r, 0] - want).abs().max()) <= 2.0 ** -7 * 6, (size, sign, r)
