@@ -38,6 +38,19 @@ template <> struct El<float> {
 // sum, values and m go together -- but that no probability passes 2^15: far scores, of which 14 is within a rounding or two, go unlifted.)
 template <typename T> __device__ __forceinline__ float reference_of(float mx) { return El<T>::LIFT != 0.f && fabsf(mx) < 0x1p20f ? mx - El<T>::LIFT : mx; }
 
+// A probability's exponent is one fused c score - m, while m came from a rounded product: of scores past 2^28 the two are 16 and more
+// apart, and the largest probability left the range of a half, past 2^31 that of a float (NaN, or a sum of 0).  From FAR on -- the rounding is
+// then half of one -- the product is rounded as m's was, so that the largest score's exponent is 0.
+constexpr float FAR = 0x1p24f;
+template <int N, typename V> __device__ __forceinline__ void settle(V& s, float c, float m) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float x = s[i] * c;
+        asm volatile("" : "+v"(x));              // (or the compiler fuses it all the same)
+        s[i] = x - m;
+    }
+}
+
 struct Args {
     const void* q; int64_t q_row, q_head;
     void* out; int64_t o_row, o_head;
@@ -288,8 +301,10 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
                 m = m_new;
             }
             // (fused: the rounding of the running maximum is common to all probabilities, a score's own product is not rounded)
+            float c2 = a.c, from = base;
+            if (__any(fabsf(base) >= FAR)) { settle<4>(sc[0], c2, from); settle<4>(sc[1], c2, from); c2 = 1.f; from = 0.f; }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], a.c, -base));
+            for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], c2, -from));
             // A value that is no number may sit in a row that some queries do not see, and 0 * NaN would reach them.  Where a
             // turn is masked at all its values are looked at: such elements leave the operands, and enter below one key at a
             // time, for the queries that see it.
@@ -762,10 +777,12 @@ __global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_ker
                         for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
                         m = m_new;
                     }
+                    float c2 = a.c_abs, from = base;
+                    if (__any(fabsf(base) >= FAR)) { settle<16>(sc, c2, from); c2 = 1.f; from = 0.f; }
                     vec pf[2];
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], a.c_abs, -base));
+                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[r], c2, -from));
                         l += p;
                         pf[r >> 3][r & 7] = (T)p;
                     }

@@ -154,3 +154,31 @@ def test_scores_far_from_zero(H, dt, nq, size):
                 p = torch.softmax(s[r, :seen], 0)
                 want = p @ b.rows_v[0][:seen, 0]
                 assert float((got[r, 0] - want).abs().max()) <= 2.0 ** -7 * 6, (size, sign, r)
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+@pytest.mark.parametrize("nq", [1, 80])
+@pytest.mark.parametrize("page", [16, 7])
+def test_scores_past_what_a_float_tells_apart(H, dt, nq, page):
+    """Scores of 10^9 .. 10^12, whose fused product and the rounded one they are taken from are hundreds apart: still an average of values,
+    that of the largest score where it stands clear of the others."""
+    for D in (64, 480):
+        for sign in (1.0, -1.0):
+            for size in (10000.0, 60000.0) + ((1e6,) if dt != "f16" else ()):
+                n, top = 150, 40
+
+                def keys(i):
+                    k = torch.full((n, 1, D), -sign * size, device="cuda")
+                    k[top] = sign * size if sign > 0 else -0.5 * sign * size
+                    return k
+
+                q = torch.full((nq, 1, D), size, device="cuda")
+                q[..., ::3] *= 0.77
+                b = Made(TYPES[dt], [n], [nq], 1, 1, D, page, keys=keys, queries=q, seed=6)
+                got = b.run(H).double()
+                s = (b.q[:, 0].double() @ b.rows_k[0][:, 0].T)
+                for r in range(nq):
+                    seen = n - nq + r + 1
+                    tie = s[r, :seen] == s[r, :seen].max()          # one key, or all the others: equal rows
+                    want = b.rows_v[0][:seen, 0][tie].mean(0)
+                    assert float((got[r, 0] - want).abs().max()) <= 2.0 ** -7 * 6, (D, sign, size, r)
