@@ -801,14 +801,14 @@ __global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_ker
         }
 
         // ---- values that are no numbers -------------------------------------------------------------------------------------------
-        // They may sit in rows that some queries do not see, and 0 * NaN would have reached them: where a turn is masked at all they
-        // have left the operands.  If there were any, the queries that see their keys get them here, one key at a time.
+        // They may sit in rows that some queries do not see, and 0 * NaN would have reached them: where a turn is masked at all, or has a
+        // key on no page, they have left the operands.  If there were any, the queries that see their keys get them here, one key at a time.
         if (__builtin_amdgcn_readfirstlane(*s_odd)) {
             for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
                 const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n);
                 for (int x = (int)x0; x < x1; ++x) {
-                    const int xb = (int)x0 + (x - (int)x0) / KT * KT;
-                    if (xb >= wg_lo && xb + KT <= min(wg_hi, x1)) continue;
+                    const int u = (x - (int)x0) / KT, xb = (int)x0 + u * KT;
+                    if (xb >= wg_lo && xb + KT <= min(wg_hi, x1) && !__any(cache_row(a, s, t.kb + xb + lane % KT) == BAD)) { x = xb + KT - 1; continue; }
                     const unsigned row = __builtin_amdgcn_readfirstlane(cache_row(a, s, t.kb + x));
                     if (row == BAD) continue;
                     const T *vp = vbase + cache_offset(a, row), *kp = kbase + cache_offset(a, row);

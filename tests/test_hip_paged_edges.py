@@ -182,3 +182,38 @@ def test_scores_past_what_a_float_tells_apart(H, dt, nq, page):
                     tie = s[r, :seen] == s[r, :seen].max()          # one key, or all the others: equal rows
                     want = b.rows_v[0][:seen, 0][tie].mean(0)
                     assert float((got[r, 0] - want).abs().max()) <= 2.0 ** -7 * 6, (D, sign, size, r)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,D", [(2, 2, 64), (4, 2, 128), (2, 2, 150), (1, 1, 256), (2, 1, 40), (1, 1, 200)])
+@pytest.mark.parametrize("page", [16, 10, 64])
+def test_missing_pages_in_chunks(H, dt, heads, kv, D, page):
+    """Table entries that name no page, in turns that every row sees and in the diagonal ones; then with NaN and infinity in rows of pages
+    that are there, beside the missing ones: they reach the queries that see them, and no others."""
+    n, nq = 500, 170
+    b = Batch(TYPES[dt], [n, 90], [nq, 90], heads, kv, D, page, seed=D + page)
+    table, gone = b.table.clone(), (100 // page, (n - 60) // page)
+    table[0, gone[0]], table[0, gone[1]], table[1, 30 // page] = -1, 10 ** 6, b.k.shape[0]
+    b.table = table
+
+    def blind(i, pos):
+        p = pos // page
+        return (p == gone[0]) | (p == gone[1]) if i == 0 else p == 30 // page
+
+    got = b.run(H)
+    want, tol = b.want(blind=blind)
+    assert bool(((got.double() - want).abs() <= tol).all())
+    # a value beside the first gap (seen by all rows), one beside the second (by the last ones)
+    beside = [gone[0] * page - 1, (gone[1] + 1) * page]
+    for what in (math.nan, math.inf):
+        for pos in beside:
+            pg, keep = int(table[0, pos // page]), b.v[int(table[0, pos // page]), pos % page].clone()
+            b.v[pg, pos % page, :, D // 3] = what
+            odd = b.run(H)
+            b.v[pg, pos % page] = keep
+            sees = torch.arange(n - nq, n, device="cuda") >= pos
+            hit = odd[:nq, :, D // 3].float()
+            assert bool((~torch.isfinite(hit[sees])).all()), (what, pos)
+            clean = torch.ones_like(odd, dtype=torch.bool)
+            clean[:nq][sees, :, D // 3] = False
+            assert bool(((odd.double() - want).abs() <= tol)[clean].all()), (what, pos)
