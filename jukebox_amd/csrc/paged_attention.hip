@@ -15,6 +15,7 @@ template <> struct El<f16> {
     static constexpr int E = 8;
     static constexpr unsigned ABS = 0x7fff7fffu, STEP = 0x04000400u;      // of two elements: without the sign; the exponent's lowest bit
     static constexpr float LIFT = 14.f;                                   // see reference_of
+    static constexpr float TINY = 0x1p-24f, SPLIT = 0x1p-13f;             // the smallest number; from where on a half of one is exact
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct El<bf16> {
@@ -22,6 +23,7 @@ template <> struct El<bf16> {
     static constexpr int E = 8;
     static constexpr unsigned ABS = 0x7fff7fffu, STEP = 0x00800080u;
     static constexpr float LIFT = 0.f;
+    static constexpr float TINY = 0x1p-126f, SPLIT = 0x1p-125f;
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct El<float> {
@@ -50,6 +52,10 @@ template <int N, typename V> __device__ __forceinline__ void settle(V& s, float 
         s[i] = x - m;
     }
 }
+
+// A number's part that is left to the first of two places; what is missing goes to the second.  Both are exact, and of the number's own sign
+// unless it is 0, or no larger than the smallest (bf16: normal) one.
+template <typename T> __device__ __forceinline__ float half_of(float v) { return fabsf(v) >= El<T>::SPLIT ? v * 0.5f : v == 0.f ? 0.f : v - copysignf(El<T>::TINY, v); }
 
 struct Args {
     const void* q; int64_t q_row, q_head;
@@ -177,6 +183,59 @@ template <typename T> __device__ __forceinline__ void store8(T* o, const float* 
     *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, x);
 }
 
+// Values that are no numbers, for the 16 rows of a tile from row0 on that are not in `skip`: where a row sees an infinite value its output is
+// infinite, where it sees infinite ones of both signs or a NaN it is no number, whatever else is in the sum (a probability is never 0).  The
+// matrix products cannot say so: a value a row does not see would reach it as 0 * NaN, and one that it sees meets parts that are 0 -- the low
+// part of a probability that has none, a probability that rounds to 0.  So turns that some row does not see whole take such values out of
+// the operands, and a tile that has met one, or whose sums are not finite, ends here: one wave looks through the split's values, 64
+// keys at a time, for those that are no numbers, and overwrites what they decide.  Channels dc .. dc + 63 for dc = 64 part, + 64 parts, ...
+template <typename T>
+__device__ void put_infinities(const Args& a, const Seq& s, const Tile& t, int kvh, int split, int n_act, int row0, unsigned skip, int part, int parts) {
+    constexpr int E = El<T>::E;
+    const int lane = threadIdx.x & 63, my = min(row0 + (lane & 15), t.rows - 1), D = a.D;
+    const T* vbase = (const T*)a.v + (int64_t)kvh * a.head_stride;
+    int first, end;
+    {
+        const int p = s.pos0 + t.j0 + (int)jb_div(my, a.group) * t.js;
+        sees(a, p, first, end);
+        if (t.ks == 1) { first = max(first - t.kb, 0); end -= t.kb; }
+        else { first = 0; end = p < 0 ? 0 : p / t.ks + 1; }
+    }
+    for (int dc = part * 64; dc < D; dc += parts * 64) {
+        unsigned pos = 0u, neg = 0u;             // bit r: row r sees such a value of channel dc + lane
+        for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
+            const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n);
+            for (int xb = (int)x0; xb < x1; xb += 64) {
+                const unsigned rows = cache_row(a, s, t.kb + min(xb + lane, x1 - 1) * t.ks);         // a key a lane
+                bool odd = false;
+                if (rows != BAD && xb + lane < x1)
+                    for (int d = dc; d < min(dc + 64, D); d += E) {
+                        const u32x4 w = load16(vbase + cache_offset(a, rows) + min(d, D - E));
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) odd |= (((w[h] & El<T>::ABS) + El<T>::STEP) & ~El<T>::ABS) != 0u;
+                    }
+                for (unsigned long long who = __ballot(odd); who; who &= who - 1) {
+                    const int i = __builtin_ctzll(who), x = xb + i;
+                    const float v = (float)vbase[cache_offset(a, (unsigned)__builtin_amdgcn_readlane((int)rows, i)) + min(dc + lane, D - 1)];
+                    const unsigned who_sees = (unsigned)__ballot(lane < 16 && x >= first && x < end);
+                    pos |= v != v || v == INFINITY ? who_sees : 0u;
+                    neg |= v != v || v == -INFINITY ? who_sees : 0u;
+                }
+            }
+        }
+        if (dc + lane >= D) continue;
+        for (int r = 0; r < 16; ++r) {
+            const bool up = pos >> r & 1u, down = neg >> r & 1u;
+            if (skip >> r & 1u || !(up || down)) continue;
+            const float v = up && down ? NAN : up ? INFINITY : -INFINITY;
+            const int i = (int)jb_div(row0 + r, a.group), h = kvh * a.G + (row0 + r - i * a.G);
+            const int64_t tok = s.t0 + t.j0 + i * t.js;
+            if (n_act > 1) a.part[((tok * a.n_head + h) * a.splits + split) * (int64_t)D + dc + lane] = v;
+            else ((T*)a.out)[tok * a.o_row + (int64_t)h * a.o_head + dc + lane] = (T)v;
+        }
+    }
+}
+
 // One workgroup per (sequence, kv head, tile of 16 rows, split of the keys).
 //
 //   S^T = K Q^T     A = 16 keys x 32 channels straight from the cache rows, B = the rows' queries (in registers throughout): a
@@ -200,10 +259,11 @@ template <typename T> __device__ __forceinline__ void store8(T* o, const float* 
 // instead of ALIGNED: 345, 70 and 350 us.
 template <typename T, int NC> struct Shape {
     static constexpr int WAVES = NC > 4 ? NC : 4, KG = WAVES / NC, CH = 16 * El<T>::E, LDO = CH + 4;     // LDO: rows 4 banks apart
-    struct Shared {
+    struct alignas(16) Shared {
         float s[NC > 1 ? 2 : 1][NC > 1 ? WAVES : 1][NC > 1 ? 64 : 1][8];      // parts of the scores, two turns' worth
         float o[KG > 1 ? WAVES : 1][KG > 1 ? 16 : 1][LDO];
         float ml[KG][16][2];
+        int odd;
     };
 };
 template <typename T, int NC, bool ALIGNED>
@@ -271,9 +331,26 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;            // of the lane's row: the reference the same in its four lanes, the sum a part in each
+        bool odd = false;                        // values that are no numbers have been taken out of a turn (put_infinities)
+        // Channels that a fragment past the head's end has over again meet zeros of the query: out of the keys they go too (an infinite one
+        // would be 0 * inf, not the score of -inf that takes its key out)
+        const bool tail = NC == 1 ? D < CH : nk > 0 && D - cb < nk * KT;
+        auto clear_tail = [&](u32x4 (&kf)[2][NK]) {
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) {
+                if (ks < nk - 1) continue;
+                const int again = cb + ks * KT + g * E - (D - E);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const unsigned keep = E == 4 ? (again > d ? 0u : ~0u) : again >= 2 * d + 2 ? 0u : again == 2 * d + 1 ? 0xffff0000u : ~0u;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) kf[h][ks][d] &= keep;
+                }
+            }
+        };
 
         // One turn: the scores' parts so far in sc, the values in vf.  gone: bit i, no page holds key i.
-        auto turn = [&](f32x4 (&sc)[2], u32x4 (&vf)[8], int xb, int x1, unsigned gone, auto value_row) {
+        auto turn = [&](f32x4 (&sc)[2], u32x4 (&vf)[8], int xb, int x1, unsigned gone) {
             // scores of keys h * 16 + g * 4 + r, i.e. of slot i = h * 4 + r
             const bool masked = xb + KB > x1 || xb < all_lo || xb + KB > all_hi || __any(gone != 0u);
             unsigned see = 0xffu;
@@ -305,26 +382,21 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
             if (__any(fabsf(base) >= FAR)) { settle<4>(sc[0], c2, from); settle<4>(sc[1], c2, from); c2 = 1.f; from = 0.f; }
 #pragma unroll
             for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], c2, -from));
-            // A value that is no number may sit in a row that some queries do not see, and 0 * NaN would reach them.  Where a
-            // turn is masked at all its values are looked at: such elements leave the operands, and enter below one key at a
-            // time, for the queries that see it.
-            unsigned odd = 0u;
+            // Where a turn is masked at all its values are looked at: those that are no numbers leave the operands.
             if (masked) {
                 const unsigned left = (unsigned)max(x1 - xb - g * 4, 0);       // keys that are there at all: before the end, on a page
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     p[i] = see >> i & 1u ? p[i] : 0.f;
                     const unsigned there = (unsigned)((i >> 2) * 16 + (i & 3)) < left && !(gone >> i & 1u) ? 0xffffffffu : 0u;
-                    unsigned any = 0u;
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         const unsigned w = vf[i][h] & there;
                         // the top bit of an element: all of its exponent's are set (an addition carries into it)
                         const unsigned bad = ((w & El<T>::ABS) + El<T>::STEP) & ~El<T>::ABS;
                         vf[i][h] = w & ~(E == 8 ? (bad - (bad >> 15)) | bad : (unsigned)((int)bad >> 31));
-                        any |= bad;
+                        odd |= bad != 0u;
                     }
-                    odd |= (any != 0u ? 1u : 0u) << i;
                 }
             }
 #pragma unroll
@@ -346,29 +418,6 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
 #pragma unroll
                     for (int e = 0; e < E; ++e)
                         acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, vf[i])[e], p[i], acc[e], 0, 0, 0);
-            }
-            if (__any(odd != 0u)) {
-                for (int i = 0; i < 8; ++i) {
-                    const unsigned long long who = __ballot(odd >> i & 1u);
-                    float pi = p[0];
-#pragma unroll
-                    for (int u = 1; u < 8; ++u) pi = u == i ? p[u] : pi;
-                    for (int gg = 0; gg < 4; ++gg) {
-                        if ((who >> (16 * gg) & 0xffffull) == 0) continue;
-                        const float pk = __shfl(pi, gg * 16 + c);
-                        const bool take = __shfl(see, gg * 16 + c) >> i & 1u;
-                        const T* vp = value_row(i, gg);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const vec w = __builtin_bit_cast(vec, load16(vp + min(cb + (g * 4 + r) * E, D - E)));
-#pragma unroll
-                            for (int e = 0; e < E; ++e) {
-                                const float x = (float)w[e];
-                                if (take && !(fabsf(x) < INFINITY)) acc[e][r] += pk * x;
-                            }
-                        }
-                    }
-                }
             }
         };
         // the slices' parts of a turn's scores, added up in the same order by all: their statistics are the same bit for bit
@@ -431,6 +480,7 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
                     const bool on = xb < x1;
                     f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
                     if (on) {
+                        if (tail) clear_tail(kf);
 #pragma unroll
                         for (int ks = 0; ks < NK; ++ks)
                             if (NC == 1 || ks < nk) {
@@ -441,10 +491,9 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
                     // the next turn's keys take the registers of this one's, and are on their way while it goes on; its values later
                     // those of this one's
                     const unsigned lost = gone;
-                    const int64_t at[2] = {row_at[0], row_at[1]};
                     if (u + 1 < turns) { find(u + 1); load_k(); }
                     if constexpr (NC > 1) add_slices(sc, on);
-                    if (on) turn(sc, vf, xb, x1, lost, [&](int i, int gg) { return vbase + at[i >> 2] + (int64_t)(gg * 4 + (i & 3)) * a.row_stride; });
+                    if (on) turn(sc, vf, xb, x1, lost);
                     if (u + 1 < turns) load_v();
                 }
             } else {
@@ -478,6 +527,7 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
                         // the next turn's rows are looked up meanwhile
                         const int xn = xb + KG * KB;
                         if (xn < x1) row = cache_row(a, s, t.kb + min(xn + (lane & 31), x1 - 1) * t.ks);
+                        if (tail) clear_tail(kf);
 #pragma unroll
                         for (int ks = 0; ks < NK; ++ks)
                             if (NC == 1 || ks < nk) {
@@ -486,12 +536,7 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
                             }
                     }
                     if constexpr (NC > 1) add_slices(sc, on);
-                    if (on) turn(sc, vf, xb, x1, gone, [&](int i, int gg) {
-                        unsigned r = vrow[0];
-#pragma unroll
-                        for (int q = 1; q < 8; ++q) r = q == i ? vrow[q] : r;
-                        return vbase + cache_offset(a, __shfl(r, gg * 16));
-                    });
+                    if (on) turn(sc, vf, xb, x1, gone);
                 }
             }
         }
@@ -502,6 +547,7 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
         if constexpr (KG > 1) {
             __syncthreads();                      // the exchange of the previous tile has been read
             if (g == 0 && cb == 0) { sh.ml[kg][c][0] = m; sh.ml[kg][c][1] = l; }
+            if (threadIdx.x == 0) sh.odd = 0;
             __syncthreads();
             M = -INFINITY; L = 0.f;
 #pragma unroll
@@ -511,6 +557,15 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
             for (int w = 0; w < KG; ++w) L += sh.ml[w][c][1] * __builtin_amdgcn_exp2f(sh.ml[w][c][0] - base);
             mine = __builtin_amdgcn_exp2f(m - base);
         }
+        const bool counts = row_ok && L > 0.f;    // (a sum that is no number, of the scores, has outputs that are none)
+        float zero = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) zero = fmaf(acc[e][r], 0.f, zero);         // or no number
+        odd |= counts && zero != 0.f;
+        if constexpr (KG > 1) { if (odd) sh.odd = 1; }
+        else odd = __syncthreads_or(odd);
         // a state of several is joined with the others' by its own maximum and sum; nothing seen: zeros
         mine *= n_act > 1 ? 1.f : L != 0.f ? 1.f / L : 0.f;
         if (n_act > 1 && wave == 0 && g == 0 && row_ok) {
@@ -545,6 +600,7 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
                 for (int e = 0; e < E; e += 4)
                     *reinterpret_cast<f32x4*>(&sh.o[wave][c][(g * 4 + r) * E + e]) = f32x4{acc[e][r], acc[e + 1][r], acc[e + 2][r], acc[e + 3][r]} * mine;
             __syncthreads();
+            odd = __builtin_amdgcn_readfirstlane(sh.odd);
             const int wr = threadIdx.x >> 4, wc = threadIdx.x & 15, wR = min(t.row0 + wr, t.rows - 1), wi = (int)jb_div(wR, a.group);
 #pragma unroll
             for (int u = 0; u < NC; ++u) {
@@ -558,6 +614,10 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
                 }
                 if (t.row0 + wr < t.rows && d0 < D) put(s.t0 + t.j0 + wi * t.js, kvh * a.G + (wR - wi * a.G), min(d0, D - E), v);
             }
+        }
+        if (odd) {
+            __syncthreads();
+            put_infinities<T>(a, s, t, kvh, split, n_act, t.row0, ~(unsigned)__ballot(counts), wave, Sh::WAVES);
         }
     }
 }
@@ -643,6 +703,22 @@ __global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_ker
                 if (at + e < e0 || R >= t.rows) x[e] = (T)0.f;
             if (a.c < 0.f) x = -x;                // (the softmax below takes a scale that is not negative)
             qf[ks] = x;
+        }
+        if (NP * 8 > D) {
+            // the channels that the last piece has over again are halved in both: with 0 in one, an infinite key would be 0 * inf there
+            vec prev = __builtin_bit_cast(vec, load16(qrow + max(NP * 8 - 16, 0))), last = __builtin_bit_cast(vec, load16(qrow + D - 8));
+            const int again = NP * 8 - D;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = a.c < 0.f ? -(float)last[e] : (float)last[e], w = a.c < 0.f ? -(float)prev[e] : (float)prev[e];
+                last[e] = (T)(e < again ? v - half_of<T>(v) : v);
+                prev[e] = (T)(e >= 8 - again ? half_of<T>(w) : w);
+            }
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) {
+                if (R < t.rows && ks * 2 + h == NP - 1) qf[ks] = last;
+                if (R < t.rows && ks * 2 + h == NP - 2) qf[ks] = prev;
+            }
         }
         // the walked keys that the lane's row sees; those that all of the wave's rows see, and any of them (a wave without rows: none)
         int xlo, xhi, all_lo = 0x7fffffff, all_hi = 0, any_lo = 0x7fffffff, any_hi = 0;
@@ -800,49 +876,17 @@ __global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_ker
             }
         }
 
-        // ---- values that are no numbers -------------------------------------------------------------------------------------------
-        // They may sit in rows that some queries do not see, and 0 * NaN would have reached them: where a turn is masked at all, or has a
-        // key on no page, they have left the operands.  If there were any, the queries that see their keys get them here, one key at a time.
-        if (__builtin_amdgcn_readfirstlane(*s_odd)) {
-            for (unsigned x0 = split * a.chunk; x0 < (unsigned)t.n; x0 += n_act * a.chunk) {
-                const int x1 = (int)min(x0 + a.chunk, (unsigned)t.n);
-                for (int x = (int)x0; x < x1; ++x) {
-                    const int u = (x - (int)x0) / KT, xb = (int)x0 + u * KT;
-                    if (xb >= wg_lo && xb + KT <= min(wg_hi, x1) && !__any(cache_row(a, s, t.kb + xb + lane % KT) == BAD)) { x = xb + KT - 1; continue; }
-                    const unsigned row = __builtin_amdgcn_readfirstlane(cache_row(a, s, t.kb + x));
-                    if (row == BAD) continue;
-                    const T *vp = vbase + cache_offset(a, row), *kp = kbase + cache_offset(a, row);
-                    bool odd = false;
-                    for (int d = lane; d < D; d += 64) odd |= !(fabsf((float)vp[d]) < INFINITY);
-                    if (!__any(odd)) continue;
-                    float dot = 0.f;
-#pragma unroll
-                    for (int ks = 0; ks < NKS; ++ks) {
-                        const vec kf = __builtin_bit_cast(vec, load16(kp + min((ks * 2 + h) * 8, D - 8)));
-                        vec q = qf[ks];
-                        asm volatile("" : "+v"(q));           // (or the queries are made single-precision for all keys at once: 128 registers)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) dot = fmaf((float)kf[e], (float)q[e], dot);
-                    }
-                    dot += __shfl_xor(dot, 32);
-                    const float pk = __builtin_amdgcn_exp2f(fmaf(dot, a.c_abs, -m));
-                    const bool take = x >= xlo && x < xhi;
-#pragma unroll
-                    for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int pc = dt * 4 + (r >> 2), e = h * 4 + (r & 3);
-                            const float v = pc < NP ? (float)vp[min(pc * 8, D - 8) + e] : 0.f;
-                            if (take && !(fabsf(v) < INFINITY)) acc[dt][r] += pk * v;
-                        }
-                }
-            }
-        }
-
         // ---- states out ---------------------------------------------------------------------------------------------------------
         const int64_t tok = s.t0 + qi;
         const float sum = l + __shfl_xor(l, 32);
         const float mine = n_act > 1 ? 1.f : sum != 0.f ? 1.f / sum : 0.f;
+        const bool counts = R < t.rows && sum > 0.f;         // (a sum that is no number, of the scores, has outputs that are none)
+        float zero[4] = {0.f, 0.f, 0.f, 0.f};     // or no numbers
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) zero[r & 3] = fmaf(acc[dt][r], 0.f, zero[r & 3]);
+        const bool odd = __builtin_amdgcn_readfirstlane(*s_odd) || __any(counts && (zero[0] + zero[1]) + (zero[2] + zero[3]) != 0.f);
         if (R < t.rows) {
             if (n_act > 1 && h == 0) {
                 float* o = a.ml + ((tok * a.n_head + head) * a.splits + split) * 2;
@@ -865,6 +909,11 @@ __global__ __launch_bounds__(256, (DP <= 160 ? 2 : 1)) void attn_paged_chunk_ker
                         for (int k = 0; k < 4; ++k) o[k] = (T)(acc[dt][r4 * 4 + k] * mine);
                     }
                 }
+        }
+        if (__builtin_expect(odd, 0)) {
+            __threadfence_block();                // (the rows' other outputs are written)
+            const unsigned skip = ~(unsigned)__ballot(counts);
+            for (int half = 0; half < 2; ++half) put_infinities<T>(a, s, t, kvh, split, n_act, R0 + half * 16, skip >> (half * 16), 0, 1);
         }
     }
 }
@@ -905,14 +954,16 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(const Args a, int 
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 if (R0 + r * tile_rows >= end) break;
-                const float M = jb_wave_max(m[r]), base = M == -INFINITY ? 0.f : M, e = __builtin_amdgcn_exp2f(m[r] - base), L = jb_wave_sum(l[r] * e);
+                // (a state weighs 2^-100 at least, so that an infinite value in it stays one; the others do not feel it)
+                const float M = jb_wave_max(m[r]), base = M == -INFINITY ? 0.f : M, e = lane < n_act ? fmaxf(__builtin_amdgcn_exp2f(m[r] - base), 0x1p-100f) : 0.f,
+                            L = jb_wave_sum(l[r] * e);
                 const float w = L != 0.f ? e / L : 0.f;
                 f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (u * 4 < n_act) {
-                        const float wu = __shfl(w, u * 4 + part_of);      // (a lane behind the last split weighs nothing)
-                        o += v[r][u] * wu;
+                        const float wu = __shfl(w, u * 4 + part_of);
+                        if (u * 4 + part_of < n_act) o += v[r][u] * wu;
                     }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[k] = jb_rows_reduce(o[k], [](float x, float y) { return x + y; });

@@ -217,3 +217,71 @@ def test_missing_pages_in_chunks(H, dt, heads, kv, D, page):
             clean = torch.ones_like(odd, dtype=torch.bool)
             clean[:nq][sees, :, D // 3] = False
             assert bool(((odd.double() - want).abs() <= tol)[clean].all()), (what, pos)
+
+
+def seen_infinities(b, func, bc):
+    """(values, tolerances) in 64 bits, product by product: infinite keys and values as the definition has them."""
+    scale, u, at = 1.0 / math.sqrt(b.D), torch.finfo(b.dtype).eps / 2, 0
+    dp = {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[b.dtype] + 2.0 ** -22
+    out = torch.zeros(b.q.shape, dtype=torch.float64, device="cuda")
+    tol = torch.full_like(out, 1e-30)
+    for i, (n, nq) in enumerate(zip(b.lens, b.nq)):
+        q = b.q[at:at + nq].double()
+        see = visible(func, bc, 0, torch.arange(n - nq, n, device="cuda")[:, None], torch.arange(n, device="cuda")[None, :])
+        for h in range(b.heads):
+            k, v = (r[i][:, h * b.kv // b.heads] for r in (b.rows_k, b.rows_v))
+            fk, fv = (torch.where(torch.isfinite(x), x, 0.0) for x in (k, v))
+            for r in range(nq):
+                s = torch.where(see[r], (q[r, h] * k).sum(1) * scale, -math.inf)
+                ds = b.D * 2.0 ** -24 * (q[r, h].abs() * fk.abs()).sum(1).max() * scale + 3 * 2.0 ** -24 * float(torch.where(torch.isfinite(s), s.abs(), 0.0).max())
+                p = torch.softmax(s, 0)
+                out[at + r, h] = torch.where(see[r][:, None] & (p != 0)[:, None], p[:, None] * v, 0.0).sum(0)
+                whole = torch.where(see[r], p, 0.0)[:, None].nan_to_num() * fv.abs()
+                tol[at + r, h] += u * out[at + r, h].abs().nan_to_num(posinf=0.0) + (2 * ds + dp + (n / 64 + 64) * 2.0 ** -24) * whole.sum(0) * (1 + u) + (
+                    2.0 ** -24 if b.dtype == torch.float16 else 0.0)
+        at += nq
+    return out, tol
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+@pytest.mark.parametrize("what", ["value", "values", "key"])
+@pytest.mark.parametrize("heads,kv,D,lens,nq,page,func,bc", [
+    (2, 2, 64, [100], [1], 16, DENSE, 0), (4, 2, 128, [100, 70], [1, 3], 16, DENSE, 0), (3, 3, 33, [90], [2], 7, DENSE, 0), (1, 1, 150, [200], [1], 16, DENSE, 0),
+    (1, 1, 250, [130], [5], 20, DENSE, 0), (1, 1, 480, [150], [1], 64, DENSE, 0), (2, 1, 300, [90], [34], 16, DENSE, 0), (2, 1, 128, [5000], [1], 16, DENSE, 0),
+    (2, 2, 64, [300], [70], 16, DENSE, 0), (2, 2, 150, [260], [66], 32, DENSE, 0), (1, 1, 40, [300], [80], 10, DENSE, 0), (4, 2, 250, [200], [40], 16, DENSE, 0),
+    (1, 1, 64, [2100], [70], 64, DENSE, 0), (2, 1, 50, [120], [90], 16, TRANSPOSE, 20)],
+    ids=["one64", "one128", "few33", "one150", "few250", "one480", "chunk300", "split", "chunk64", "chunk150", "chunk40", "chunk250", "splitchunk", "transpose"])
+def test_infinities_that_are_seen(H, dt, what, heads, kv, D, lens, nq, page, func, bc):
+    """An infinite value in an output's sum makes it infinite (two of both signs: no number); an infinite channel of a key makes its score
+    infinite: -inf takes the key out, +inf leaves no number.  Whatever the turn, the kernel, and the channel, a head's last ones too."""
+    for where in (D - 1, D - 8, D // 2, 0):
+        b = Batch(TYPES[dt], lens, nq, heads, kv, D, page, seed=D + where)
+        for pos, sign in [(5, -1.0)] + ([(8, 1.0)] if what == "values" else []):
+            pos = pos if func == DENSE else pos * bc // 5        # (the transpose pattern: positions of one residue)
+            x, rows = (b.k, b.rows_k) if what == "key" else (b.v, b.rows_v)
+            x[int(b.table[0, pos // page]), pos % page, :, where] = sign * math.inf
+            rows[0][pos, :, where] = sign * math.inf
+        got = b.run(H, func=func, block_ctx=bc).double()
+        want, tol = seen_infinities(b, func, bc)
+        nan, inf = torch.isnan(want), torch.isinf(want)
+        assert bool(torch.isnan(got).eq(nan).all()), f"{int((torch.isnan(got) != nan).sum())} of {nan.numel()} are (no) numbers, channel {where}"
+        assert torch.equal(got[inf], want[inf])
+        fine = ~nan & ~inf
+        assert bool(((got - want).abs() <= tol)[fine].all()), where
+        assert what != "value" or bool(inf.any())
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+@pytest.mark.parametrize("nats", [30.0, 75.0])
+@pytest.mark.parametrize("heads,kv,D,lens,nq,page", [(2, 2, 64, [300], [1], 16), (2, 1, 128, [6000], [1], 16), (1, 1, 480, [200], [3], 7), (1, 1, 150, [300], [80], 16), (1, 1, 64, [2100], [70], 16)],
+                         ids=["one", "split", "480", "chunk", "splitchunk"])
+def test_an_infinite_value_of_a_probability_that_is_nearly_none(H, dt, nats, heads, kv, D, lens, nq, page):
+    """e^-30 and e^-75 of an infinite value are infinite, in whatever part of the keys it lies."""
+    for pos in (5, lens[0] - 90):
+        b = peaked(dt, heads, kv, D, lens, nq, page, nats, seed=D)
+        want, tol = b.fine()
+        b.v[int(b.table[0, pos // page]), pos % page, :, D - 3] = -math.inf
+        got = b.run(H).double()
+        assert bool((got[:, :, D - 3] == -math.inf).all()), pos
+        rest = torch.arange(D, device="cuda") != D - 3
+        assert bool(((got - want).abs() <= tol)[..., rest].all()), pos
