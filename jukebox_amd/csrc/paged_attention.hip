@@ -954,16 +954,17 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(const Args a, int 
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 if (R0 + r * tile_rows >= end) break;
-                // (a state weighs 2^-100 at least, so that an infinite value in it stays one; the others do not feel it)
-                const float M = jb_wave_max(m[r]), base = M == -INFINITY ? 0.f : M, e = lane < n_act ? fmaxf(__builtin_amdgcn_exp2f(m[r] - base), 0x1p-100f) : 0.f,
-                            L = jb_wave_sum(l[r] * e);
+                const float M = jb_wave_max(m[r]), base = M == -INFINITY ? 0.f : M, e = __builtin_amdgcn_exp2f(m[r] - base), L = jb_wave_sum(l[r] * e);
                 const float w = L != 0.f ? e / L : 0.f;
                 f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (u * 4 < n_act) {
                         const float wu = __shfl(w, u * 4 + part_of);
-                        if (u * 4 + part_of < n_act) o += v[r][u] * wu;
+                        if (wu != 0.f) o += v[r][u] * wu;                // (a lane behind the last split weighs nothing)
+                        else if (u * 4 + part_of < n_act)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) o[k] += fabsf(v[r][u][k]) < INFINITY ? 0.f : v[r][u][k];      // infinite all the same
                     }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[k] = jb_rows_reduce(o[k], [](float x, float y) { return x + y; });
