@@ -1025,6 +1025,11 @@ int64_t workspace_of(const jb_attn_paged_args* p, const Plan& w) {
     return w.splits == 1 ? 0 : (int64_t)p->n_tokens * p->n_head * w.splits * (p->d_head + 2) * 4;
 }
 
+int shift_of(int page_size) {                     // ceil(log2 page_size)
+    int s = 0;
+    while (s < 31 && (1u << s) < (unsigned)page_size) ++s;
+    return s;
+}
 int check_args(const jb_attn_paged_args* a, const char* who) {
     auto bad = [&](const char* what) { jb_set_error(std::string(who) + ": " + what); return (int)JB_ERR_ARG; };
     if (!a) return bad("null pointer");
@@ -1036,9 +1041,7 @@ int check_args(const jb_attn_paged_args* a, const char* who) {
     if (a->n_tokens < 0 || a->n_seq < 0 || a->n_head <= 0 || a->n_kv_head <= 0 || a->n_head % a->n_kv_head) return bad("bad dims");
     if (a->d_head < 8 || a->d_head > 512) { jb_set_error(std::string(who) + ": heads of 8 to 512 channels"); return JB_ERR_UNSUPPORTED; }
     if (a->n_pages <= 0 || a->page_size <= 0 || a->max_pages <= 0) return bad("bad dims of the cache");
-    int sh = 0;
-    while (sh < 31 && (1 << sh) < a->page_size) ++sh;
-    if (((uint64_t)a->n_pages << sh) > 0xffffffffull || (int64_t)a->n_pages * a->page_size > 0x7fffffff) return bad("more than 2^31 cache rows");
+    if (((uint64_t)a->n_pages << shift_of(a->page_size)) > 0xffffffffull || (int64_t)a->n_pages * a->page_size > 0x7fffffff) return bad("more than 2^31 cache rows");
     if (a->page_stride < 0 || a->row_stride < 0 || a->head_stride < 0 || a->q_row_stride < 0 || a->q_head_stride < 0 || a->table_stride < 0) return bad("negative stride");
     if (a->out_head_stride < a->d_head || a->out_row_stride < a->d_head) return bad("output rows overlap");
     if (a->attn_func != JB_ATTN_DENSE && a->block_ctx <= 0) return bad("block_ctx required");
@@ -1098,7 +1101,7 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     k.page = jb_make_div((unsigned)a->page_size);
     k.group = jb_make_div((unsigned)(a->n_head / a->n_kv_head));
     k.n_pages = (unsigned)a->n_pages;
-    while ((1 << k.page_shift) < a->page_size) ++k.page_shift;
+    k.page_shift = shift_of(a->page_size);
     k.n_tokens = a->n_tokens; k.n_seq = a->n_seq; k.n_head = a->n_head; k.n_kv = a->n_kv_head; k.G = a->n_head / a->n_kv_head; k.D = a->d_head;
     k.func = a->attn_func; k.bc = a->block_ctx > 0 ? a->block_ctx : 1; k.window = a->window;
     k.tr = w.tr; k.tiles = (int)w.tiles; k.splits = w.splits; k.chunk = w.chunk;

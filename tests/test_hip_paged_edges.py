@@ -285,3 +285,18 @@ def test_an_infinite_value_of_a_probability_that_is_nearly_none(H, dt, nats, hea
         assert bool((got[:, :, D - 3] == -math.inf).all()), pos
         rest = torch.arange(D, device="cuda") != D - 3
         assert bool(((got - want).abs() <= tol)[..., rest].all()), pos
+
+
+@pytest.mark.parametrize("page", [2 ** 30 + 1, 2 ** 30 + 16, 2 ** 31 - 1])
+def test_one_page_of_more_than_2_30_rows(H, page):
+    """A page of more rows than 2^30, all of them the same one in memory (a row stride of 0): the average is the row."""
+    for dt, D, nq in (("f16", 8, 1), ("bf16", 64, 70), ("f32", 16, 2)):
+        row = torch.randn(2, 1, 1, 1, D, device="cuda").to(TYPES[dt])
+        k, v = (x.expand(1, page, 1, D) for x in row)
+        q = torch.randn(nq, 1, D, device="cuda").to(TYPES[dt])
+        ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+        got = H.attn_paged(q, k, v, ints([0]), ints(5000), ints(0, nq), max_len=5000)
+        # probabilities that sum to 1 but for their own rounding and that of 5000 / 64 + 64 additions
+        dp = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dt]
+        u = torch.finfo(TYPES[dt]).eps / 2
+        assert float(((got.double() - v[0, 0].double()).abs() / v[0, 0].double().abs()).max()) <= u + (1 + u) * (dp + (5000 / 64 + 64) * 2.0 ** -24)
