@@ -340,7 +340,8 @@ typedef struct jb_attn_paged_args {
     const int* table; int64_t table_stride; int max_pages;
     const int* lens; const int* cu_q;                  /* [n_seq], [n_seq + 1] */
     int n_tokens, n_seq, n_head, n_kv_head, d_head;    /* n_tokens: rows of q and out */
-    int max_q, max_len;                                /* the most queries / tokens of a sequence, for the shape of the launch only */
+    int max_q, max_len;                                /* the most queries / tokens of a sequence, for the shape of the launch and the choice of the
+                                                        * kernel; less than the truth costs time (max_q 0: there are no queries) */
     int block_ctx, window;
     float scale;
     void* workspace; int64_t workspace_bytes;          /* jb_attn_paged_workspace() bytes, 16-byte aligned; holds nothing between calls */

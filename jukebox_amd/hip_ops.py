@@ -396,7 +396,7 @@ def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, fun
     ps, rs, hs = kpool.stride()[:3]
     a = L.AttnPagedArgs(code, func, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0) if T > 1 else H * D,
                         out.stride(1) if H > 1 else D, kpool.data_ptr(), vpool.data_ptr(), ps, rs, hs, P, page, table.data_ptr(),
-                        table_stride, width, lens.data_ptr(), cu_q.data_ptr(), T, n, H, KV, D, T if max_q is None else min(max_q, T),
+                        table_stride, width, lens.data_ptr(), cu_q.data_ptr(), T, n, H, KV, D, T if max_q is None else min(max_q or 1, T),
                         min(width * page if max_len is None else max_len, _INT_MAX), min(block_ctx or 0, _INT_MAX), min(window or 0, _INT_MAX),
                         1.0 / math.sqrt(D) if scale is None else scale, None, 0)
     lib = L.lib()

@@ -300,3 +300,13 @@ def test_one_page_of_more_than_2_30_rows(H, page):
         dp = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dt]
         u = torch.finfo(TYPES[dt]).eps / 2
         assert float(((got.double() - v[0, 0].double()).abs() / v[0, 0].double().abs()).max()) <= u + (1 + u) * (dp + (5000 / 64 + 64) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+def test_hints_of_zero(H, dt):
+    """max_q and max_len below the truth cost time, not correctness: 0 too."""
+    b = Batch(TYPES[dt], [300, 17], [5, 17], 4, 2, 64, 16, seed=31)
+    want, tol = b.want()
+    for kw in ({"max_q": 0}, {"max_len": 0}, {"max_q": 0, "max_len": 0}):
+        got = H.attn_paged(b.q, b.k, b.v, b.table, b.len_t, b.cu, out=torch.full_like(b.q, 7.0), **kw)
+        assert bool(((got.double() - want).abs() <= tol).all()), kw
