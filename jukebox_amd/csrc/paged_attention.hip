@@ -987,6 +987,9 @@ Plan plan_of(const jb_attn_paged_args* p) {
         w.tr = 128;
     if (p->attn_func == JB_ATTN_TRANSPOSE_BLOCK) w.tiles = (int64_t)(p->max_q < bc ? p->max_q : bc) * (((p->max_q + bc - 1) / bc * G + 15) / 16);
     else w.tiles = (rows + w.tr - 1) / w.tr;
+    // 2^20 workgroups fill the chip many times over, and a launch holds 2^32 threads: what max_q asks for beyond is walked by the tiles there are
+    const int64_t most_tiles = streams < 1 << 20 ? (1 << 20) / streams : 1;
+    if (w.tiles > most_tiles) w.tiles = most_tiles;
     // keys that a tile walks at most
     w.range = p->max_len;
     if (p->attn_func == JB_ATTN_BLOCK || p->attn_func == JB_ATTN_PREV_BLOCK) w.range = bc + w.tr / G + 15;
@@ -1091,7 +1094,8 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     const int64_t need = workspace_of(a, w);
     JB_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need && (uintptr_t)a->workspace % 16 == 0), "workspace missing, too small or not aligned");
     const int64_t wgs = w.tiles * a->n_kv_head * a->n_seq;
-    JB_REQUIRE(wgs * w.splits <= 0x7fffffff, "grid too large");
+    constexpr int64_t MOST = 0xffffffffll / 512;       // workgroups of up to 512 threads that a launch holds
+    JB_REQUIRE(wgs * w.splits <= MOST, "grid too large");
     Args k = {};
     k.q = a->q; k.q_row = a->q_row_stride; k.q_head = a->q_head_stride;
     k.out = a->out; k.o_row = a->out_row_stride; k.o_head = a->out_head_stride;
@@ -1110,7 +1114,7 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     // (a lane's offset inside a 16-row half is 32 bits wide)
     k.aligned = w.tr == 16 && a->page_size % 16 == 0 && a->attn_func != JB_ATTN_TRANSPOSE_BLOCK && a->row_stride <= 0x7fffffff / 64 - 512;
     const int64_t inner = w.tiles == 1 ? k.n_kv : w.tiles, groups = wgs * w.splits / inner;
-    JB_REQUIRE((groups + 8) * inner <= 0x7fffffff, "grid too large");
+    JB_REQUIRE((groups + 8) * inner <= MOST, "grid too large");
     k.groups = (unsigned)groups; k.by_die = w.tiles == 1 ? groups >= 8 : k.n_kv % 8 == 0;
     const int64_t grid = k.by_die ? (groups + 7) / 8 * 8 * inner : groups * inner;
     if (need) {
@@ -1123,7 +1127,7 @@ extern "C" int jb_attn_paged(const jb_attn_paged_args* a, void* stream) {
     // as much as a row, 131) -- more where tiles are so few that the waves find room at once (8 tiles, 59 states: 61 -> 51)
     const int64_t room = wgs < 64 ? 1024 / wgs : 16, side = w.tr == 16 ? 16 : room < 128 ? room : 128;
     const int tile_rows = (int)(most_rows < side ? most_rows : side);
-    JB_REQUIRE(w.splits == 1 || wgs * tile_rows <= 0x7fffffff, "grid too large");
+    JB_REQUIRE(w.splits == 1 || wgs * ((tile_rows + 3) / 4) <= MOST, "grid too large");
 #define JB_ROWS(T, CH)                                                            \
     do {                                                                          \
         if (w.tr > 16) { const int rc2 = launch_chunk<T>(k, grid, s); if (rc2) return rc2; } \

@@ -310,3 +310,25 @@ def test_hints_of_zero(H, dt):
     for kw in ({"max_q": 0}, {"max_len": 0}, {"max_q": 0, "max_len": 0}):
         got = H.attn_paged(b.q, b.k, b.v, b.table, b.len_t, b.cu, out=torch.full_like(b.q, 7.0), **kw)
         assert bool(((got.double() - want).abs() <= tol).all()), kw
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+def test_hints_far_beyond_the_truth(H, dt):
+    """70000 sequences of one token, and max_q for as many: more tiles than a launch holds workgroups."""
+    n, page = 70000, 4
+    g = torch.Generator("cuda").manual_seed(20)
+    k, v = (torch.randn(n, page, 1, 8, generator=g, device="cuda").to(TYPES[dt]) for _ in range(2))
+    q = torch.randn(n, 2, 8, generator=g, device="cuda").to(TYPES[dt])
+    table = torch.arange(n, dtype=torch.int32, device="cuda").flip(0)[:, None].contiguous()
+    lens = torch.full((n,), 3, dtype=torch.int32, device="cuda")
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    want = H.attn_paged(q, k, v, table, lens, cu, max_q=1)
+    got = H.attn_paged(q, k, v, table, lens, cu, max_q=n)
+    # three values below 6, with probabilities off by their rounding in either call
+    u = torch.finfo(TYPES[dt]).eps / 2
+    assert float((got.double() - want.double()).abs().max()) <= (4 * u + 2.0 ** -18) * 6
+    # one sequence has the queries of all, in turns of the tiles that are left
+    cu[1:] = n
+    lens[0] = 3
+    first = H.attn_paged(q, k, v, table, lens, cu, max_q=n)
+    assert bool((first[:-3] == 0).all()) and bool((first[-3:].abs().sum((1, 2)) > 0).all())
