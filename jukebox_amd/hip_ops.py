@@ -371,7 +371,8 @@ def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, fun
     q (n_tokens, n_head, d_head): rows cu_q[i] .. cu_q[i + 1] - 1 are the last positions of sequence i, whose keys and values
     the cache holds already.  kpool, vpool (n_pages, page_size, n_kv_head, d_head), any strides that both share, channels
     contiguous.  table (n_seq, max_pages), lens (n_seq), cu_q (n_seq + 1): int32 on the GPU.  max_q, max_len: the most queries
-    / tokens of a sequence, which shape the launch (default: all rows of q, all of the table's pages).  func, block_ctx: the
+    / tokens of a sequence, which shape the launch and choose the kernel.  Default: all of the table's pages; all rows of q, but 1
+    where q has a row a sequence.  func, block_ctx: the
     pattern (dense, block, transpose, prev); window: the query at position p sees p - window + 1 .. p (dense).  scale:
     1 / sqrt(d_head) by default.  Returns (n_tokens, n_head, d_head); `out` overlaps no input, and its rows outside every sequence
     stay as they are.
@@ -394,9 +395,11 @@ def attn_paged(q, kpool, vpool, table, lens, cu_q, max_q=None, max_len=None, fun
     if q.stride(2) != 1 or kpool.stride(3) != 1 or out.stride(2) != 1:
         raise L.JukeboxHipError("expected contiguous channels")
     ps, rs, hs = kpool.stride()[:3]
+    if max_q is None:   # as many rows as sequences: a step of one token each (64 of 4000 tokens, 32 heads on 8: 213 us; as a chunk 339)
+        max_q = 1 if T == n else T
     a = L.AttnPagedArgs(code, func, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0) if T > 1 else H * D,
                         out.stride(1) if H > 1 else D, kpool.data_ptr(), vpool.data_ptr(), ps, rs, hs, P, page, table.data_ptr(),
-                        table_stride, width, lens.data_ptr(), cu_q.data_ptr(), T, n, H, KV, D, T if max_q is None else min(max_q or 1, T),
+                        table_stride, width, lens.data_ptr(), cu_q.data_ptr(), T, n, H, KV, D, min(max_q or 1, T),
                         min(width * page if max_len is None else max_len, _INT_MAX), min(block_ctx or 0, _INT_MAX), min(window or 0, _INT_MAX),
                         1.0 / math.sqrt(D) if scale is None else scale, None, 0)
     lib = L.lib()

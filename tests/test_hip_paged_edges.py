@@ -44,13 +44,15 @@ class Made(Batch):
 
     def chunks(self, func, max_q=None):
         """Whether the call takes the kernel of chunks."""
-        rows = (sum(self.nq) if max_q is None else max_q) * self.heads // self.kv
+        if max_q is None:
+            max_q = 1 if sum(self.nq) == len(self.nq) else sum(self.nq)
+        rows = max_q * self.heads // self.kv
         return self.dtype != torch.float32 and func != TRANSPOSE and self.D <= 256 and rows >= 64
 
     def fine(self, func=DENSE, bc=0, window=0, max_q=None):
         """(values, tolerances) in 64 bits."""
         scale, u, at = 1.0 / math.sqrt(self.D), torch.finfo(self.dtype).eps / 2, 0
-        half, two = self.dtype == torch.float16, not self.chunks(func, max_q)
+        half, two = self.dtype == torch.float16, not Made.chunks(self, func, max_q)
         dp = {torch.float32: 0.0, torch.float16: 2.0 ** (-22 if two else -11), torch.bfloat16: 2.0 ** (-16 if two else -8)}[self.dtype] + 2.0 ** -22
         out = torch.zeros(self.q.shape, dtype=torch.float64, device="cuda")
         tol = torch.full_like(out, 1e-30)
@@ -332,3 +334,13 @@ def test_hints_far_beyond_the_truth(H, dt):
     lens[0] = 3
     first = H.attn_paged(q, k, v, table, lens, cu, max_q=n)
     assert bool((first[:-3] == 0).all()) and bool((first[-3:].abs().sum((1, 2)) > 0).all())
+
+
+def test_a_step_without_max_q(H):
+    """One token of each of many sequences: without max_q the call is the one of few tokens (the same bits), not the one of chunks."""
+    lens = [700, 33, 5, 1200] * 16
+    for heads, kv, D in ((8, 2, 128), (2, 2, 64), (16, 1, 64)):
+        b = Batch(torch.bfloat16, lens, [1] * 64, heads, kv, D, 16, seed=40)
+        assert torch.equal(b.run(H), b.run(H, max_q=1))
+        want, tol = Made.fine(b)
+        assert bool(((b.run(H).double() - want).abs() <= tol).all())
