@@ -18,4 +18,19 @@ static inline JbDiv jb_make_div(unsigned d) {
     while (s < 31 && (1u << s) < d) ++s;
     return JbDiv{d, (unsigned)((((uint64_t)1 << 32) * (((uint64_t)1 << s) - d)) / d + 1), s};
 }
+// Whether no two of n1 x n2 x n3 rows of `len` elements, at these strides, share one -- of strides that nest: each at least what the smaller ones span
+// (dimensions of one entry do not count).
+static inline bool jb_apart(int64_t len, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t n3 = 1, int64_t s3 = 0) {
+    int64_t n[3] = {n1, n2, n3}, s[3] = {s1, s2, s3}, span = len;
+    for (int done = 0; done < 3; ++done) {
+        int least = -1;
+        for (int i = 0; i < 3; ++i)
+            if (n[i] > 1 && (least < 0 || s[i] < s[least])) least = i;
+        if (least < 0) break;
+        if (s[least] < span) return false;
+        span += (n[least] - 1) * s[least];
+        n[least] = 1;
+    }
+    return true;
+}
 __device__ __forceinline__ unsigned jb_div(unsigned n, const JbDiv& v) { return (__umulhi(v.m, n) + n) >> v.s; }

@@ -1046,7 +1046,8 @@ int check_args(const jb_attn_paged_args* a, const char* who) {
     if (a->n_pages <= 0 || a->page_size <= 0 || a->max_pages <= 0) return bad("bad dims of the cache");
     if (((uint64_t)a->n_pages << shift_of(a->page_size)) > 0xffffffffull || (int64_t)a->n_pages * a->page_size > 0x7fffffff) return bad("more than 2^31 cache rows");
     if (a->page_stride < 0 || a->row_stride < 0 || a->head_stride < 0 || a->q_row_stride < 0 || a->q_head_stride < 0 || a->table_stride < 0) return bad("negative stride");
-    if (a->out_head_stride < a->d_head || a->out_row_stride < a->d_head) return bad("output rows overlap");
+    if (a->out_head_stride < a->d_head || a->out_row_stride < a->d_head ||
+        !jb_apart(a->d_head, a->n_tokens, a->out_row_stride, a->n_head, a->out_head_stride)) return bad("output rows overlap");
     if (a->attn_func != JB_ATTN_DENSE && a->block_ctx <= 0) return bad("block_ctx required");
     if (a->window < 0 || (a->window && a->attn_func != JB_ATTN_DENSE)) return bad("a window goes with the dense pattern");
     if (a->max_q < 0 || a->max_len < 0 || (int64_t)a->max_q * a->n_head > 0x7fffffff || (int64_t)a->n_tokens * a->n_head > 0x7fffffff) return bad("bad dims");

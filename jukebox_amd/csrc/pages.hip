@@ -387,6 +387,7 @@ extern "C" int jb_kv_write(const jb_kv_write_args* a, void* stream) {
     JB_REQUIRE(a->n_tokens >= 0 && a->n_kv_head > 0 && a->d_head > 0 && a->n_pages > 0 && a->page_size > 0, "bad dims");
     JB_REQUIRE(a->tok_stride >= 0 && a->tok_head_stride >= 0 && a->page_stride >= 0 && a->row_stride >= 0 && a->head_stride >= 0, "negative stride");
     JB_REQUIRE((int64_t)a->n_pages * a->page_size <= 0x7fffffff, "more than 2^31 cache rows");
+    JB_REQUIRE(jb_apart(a->d_head, a->n_pages, a->page_stride, a->page_size, a->row_stride, a->n_kv_head, a->head_stride), "rows of the cache overlap");
     const int e = a->dtype == JB_F32 ? 4 : 2;
     int64_t heads = a->n_kv_head, d = a->d_head;
     if (a->tok_head_stride == d && a->head_stride == d) { d *= heads; heads = 1; }       // the heads of a row lie together on both sides
