@@ -94,7 +94,7 @@ struct ExtendArgs {
     int n_seq, n_pages, n_tokens;
     JbDiv page;
 };
-__device__ __forceinline__ int pages_of(int len, const JbDiv& page) { return (int)jb_div((unsigned)len + page.d - 1u, page); }
+__device__ __forceinline__ int pages_of(int len, const JbDiv& page) { return len > 0 ? (int)jb_div((unsigned)len - 1u, page) + 1 : 0; }
 
 __device__ __forceinline__ void extend_token(const ExtendArgs& a, int t) {
     const int *was = a.work + 1, *first = was + a.n_seq, *found = first + a.n_seq;
