@@ -377,6 +377,7 @@ unsigned copy_grid(int64_t page_bytes, int64_t n, int pools) {
     return (unsigned)(turns < 1 ? 1 : turns > 2048 ? 2048 : turns);
 }
 constexpr int MAX_PAGES = 1 << 20;                    // sums over NT sequences' pages stay below 2^31
+constexpr int MAX_SCAN = 1 << 30;                     // pages that one workgroup scans, whose steps stay below 2^31
 constexpr int MAX_SEQS = 1 << 17;                     // rows of a table: a bit each in LDS
 
 }  // namespace
@@ -461,6 +462,7 @@ extern "C" int jb_pages_fork(const jb_page_table* t, const jb_page_pools* p, con
     JB_REQUIRE(t->table_stride >= t->max_pages || t->n_seq < 2, "rows of the table overlap");
     JB_REQUIRE((int64_t)t->n_pages * t->page_size <= 0x7fffffff, "more than 2^31 cache rows");
     JB_REQUIRE(t->n_seq <= MAX_SEQS && n_pairs <= t->n_seq, "more pairs than the table has rows, or a table of more than 131072");
+    if (t->n_pages > MAX_SCAN) JB_UNSUPPORTED("more than 2^30 pages");
     if (n_pairs == 0) return JB_OK;
     ForkArgs a = {t->table, t->table_stride, t->max_pages, t->lens, t->ref, src, dst, status, work, n_pairs, t->n_seq, t->n_pages, jb_make_div((unsigned)t->page_size)};
     hipStream_t s = (hipStream_t)stream;
@@ -480,6 +482,7 @@ extern "C" int jb_pages_compact(const jb_page_table* t, const jb_page_pools* p, 
     JB_REQUIRE(t->n_seq >= 0 && t->max_pages > 0 && t->n_pages > 0 && t->n_pages == p->n_pages, "bad dims");
     JB_REQUIRE(t->table_stride >= t->max_pages || t->n_seq < 2, "rows of the table overlap");
     JB_REQUIRE(table_out != t->table && ref_out != t->ref, "the outputs are arrays of their own");
+    if (t->n_pages > MAX_SCAN) JB_UNSUPPORTED("more than 2^30 pages");
     hipStream_t s = (hipStream_t)stream;
     pages_compact_plan_kernel<<<1, NT, 0, s>>>(t->ref, t->n_pages, work);
     JB_CHECK_LAUNCH();

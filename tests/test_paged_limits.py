@@ -50,3 +50,11 @@ def test_pools_whose_rows_overlap_are_not_written(lib):  # noqa: F811
     # (a pool made by expand, heads inside one another, pages that share their last row)
     for kw in ({"page_stride": 0}, {"row_stride": 0}, {"head_stride": 64}, {"row_stride": 128}, {"page_stride": 4095}, {"head_stride": 2047, "row_stride": 128}):
         assert write(**kw) == ERR_ARG and b"overlap" in lib.jb_last_error(), kw
+
+
+def test_more_pages_than_a_scan_counts(lib):  # noqa: F811
+    from jukebox_amd import _lib as L
+    for n, rc in (((1 << 30) + 1, -2), ((1 << 31) - 1, -2)):
+        t, p = L.PageTable(PTR, 4, 3, 4, PTR, PTR, n, 1), L.PagePools((L.vp * 1)(PTR), 1, n, 512, 512)
+        assert lib.jb_pages_fork(C.byref(t), C.byref(p), PTR, PTR, 0, PTR, PTR, None) == rc and b"2^30" in lib.jb_last_error()
+        assert lib.jb_pages_compact(C.byref(t), C.byref(p), PTR + 16, PTR + 32, PTR, None) == rc and b"2^30" in lib.jb_last_error()
