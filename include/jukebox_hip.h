@@ -292,8 +292,9 @@ int jb_sample_step(const float* logits, int n_batch, int bins, const jb_sample_p
  * which the weights sum to at most p of theirs (p <= 0 or >= 1: off); min-p those with w_i >= min_p (<= 0: off; above 1 is 1).
  * The token is the first index at which the sum of kept weights, by rising index, exceeds u times their total.  temp <= 0: the
  * largest logit, the lowest index of equal ones.  -inf and NaN are forbidden tokens; a row of nothing else gives -1.  u below 0 (NaN)
- * counts as 0, from 1 on as the last kept token.  Weights and sums are exact to 2^-45 of the largest weight: the answer is the
- * definition's in 64 bits, whatever the order of summation; weights below 2^-45 (logits 31.2 temp under the largest) are 0. */
+ * counts as 0, from 1 on as the last kept token.  Weights are whole multiples of 2^-44 of the largest, off by 0.6 of one at most, and
+ * sums of them are exact whatever the order: the answer is the definition's in 64 bits, but where a border -- u times the total, p times
+ * the sum, min-p -- lies within that error of a weight or sum; weights below 2^-45 (logits 31.2 temp under the largest) are 0. */
 typedef struct jb_sample_filtered_args {
     int dtype;                                         /* JB_F32, JB_F16, JB_BF16 */
     const void* logits; int64_t ld; int rows, bins;    /* [rows] of ld elements, bins of them logits */

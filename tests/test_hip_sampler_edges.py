@@ -1,0 +1,50 @@
+"""GPU suite: jb_sample_filtered where its weights and settings are at their limits, against its definition in 64 bits (test_hip_sampler.py)."""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_hip_sampler import TYPES, check, definition  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def H():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from jukebox_amd import _lib, hip_ops
+    _lib.lib()          # fail loudly if the extension is missing
+    return hip_ops
+
+
+# Logit x of token 0 (token 1: 0), temperature and u such that u is 1.6e-13 .. 6e-13 of itself beside w / (1 + w), w = exp(x / temp): found by search
+# over the floats, among those whose weight lies between two entries of a table of 32 a factor of two.  A weight is a multiple of 2^-44, off by 0.6
+# of one: 1.1e-13 of weights from 0.3 on at most.
+NEAR = {"f32": ["-0x1.b1ae2cp-5 0x1p+0 0x1.f2735ep-2", "-0x1.b81416p-5 0x1p+0 0x1.f24038p-2", "-0x1.c06ce8p-5 0x1p+0 0x1.f1fd7ep-2",
+                "-0x1.32fbe4p-4 0x1p+0 0x1.ecd28ep-2", "-0x1.35563ep-4 0x1p+0 0x1.ecacf6p-2", "-0x1.8f3ed8p-4 0x1p+0 0x1.e71120p-2",
+                "-0x1.8f7a1cp-4 0x1p+0 0x1.e70d6ep-2", "-0x1.90c8a8p-4 0x1p+0 0x1.e6f892p-2", "-0x1.4cfed0p-3 0x1p+0 0x1.d67790p-2",
+                "-0x1.4d97b2p-3 0x1p+0 0x1.d66494p-2", "-0x1.7945c4p-3 0x1p+0 0x1.d0f94ep-2"],
+        "bf16": ["-0x1p+0 0x1.0fa296p+0 0x1.1f232ap-2", "-0x1p+0 0x1.2baacap+0 0x1.31b34ep-2", "-0x1p+0 0x1.bdf1bap+0 0x1.70f274p-2",
+                 "-0x1p+0 0x1.d08ff2p+0 0x1.7664ecp-2"],
+        "f16": ["-0x1.90c0p-1 0x1.2fe8f6p+0 0x1.5d12b0p-2", "-0x1.90c0p-1 0x1.8910acp+0 0x1.804086p-2", "-0x1.90c0p-1 0x1.891e26p+0 0x1.8044b8p-2",
+                "-0x1.90c0p-1 0x1.ae0e9ep+0 0x1.8ad5b4p-2"]}
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+@pytest.mark.parametrize("V", [2, 3000, 20000, 70000])
+def test_numbers_next_to_a_border(H, dt, V):
+    """The draw, and min-p and top-p at the same weight: on the definition's side of the border, in rows of either size of workgroup."""
+    rows = [tuple(float.fromhex(v) for v in r.split()) for t in ("f32", "bf16", "f16") for r in NEAR[t] if t == dt or dt == "f32"]
+    x = torch.full((len(rows), V), -math.inf)
+    x[:, 0], x[:, 1] = torch.tensor([r[0] for r in rows]), 0.0
+    x = x.to(TYPES[dt])
+    assert x[:, 0].double().tolist() == [r[0] for r in rows]
+    u, temp = (torch.tensor([r[i] for r in rows]) for i in (2, 1))
+    for ui, (xi, t, _) in zip(u.tolist(), rows):
+        p = 1 / (1 + math.exp(-xi / t))
+        assert 1.5e-13 < abs(ui / p - 1) < 1e-12
+    check(H, x.cuda(), u, temp)
+    # the order is (1, 0): token 0 is kept by top-p if w(1) <= p (w(0) + w(1))
+    check(H, x.cuda(), torch.full_like(u, 0.01), temp, p=1 - u)
