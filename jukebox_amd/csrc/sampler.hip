@@ -104,12 +104,13 @@ __device__ __forceinline__ unsigned key_of(float x) { const unsigned b = __float
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
 template <typename T, bool TABLE> struct Weigh {
-    float mx, bins;                                   // largest logit; bins per unit of logit
+    float mx, bins;                                   // largest logit, bins per unit of logit: both of logits times
+    float by;                                         // a power of two, in whose scale neither differences nor bins leave a float's range
     double c, md;                                     // 32 / (T ln 2); the largest logit
     const double* tab;                                // EXP2_32 in LDS: 32 entries, one pair of banks each
     const double* keys;                               // a table of the weights themselves (see real), or NULL
     // how far below the largest, in bins; NB - 1: weighs nothing
-    __device__ __forceinline__ float depth(float x) const { return x == mx ? 0.f : fminf((mx - x) * bins, (float)(NB - 1)); }
+    __device__ __forceinline__ float depth(float x) const { return x == mx ? 0.f : fminf(fmaf(x, -by, mx * by) * bins, (float)(NB - 1)); }
     __device__ __forceinline__ int bin(float x) const { return (int)depth(x); }
     // The largest x that lies in bin b or below it (depth falls with x, also as it is rounded), so that telling an entry's bin takes
     // comparisons alone.  The whole wave: its lanes divide the interval by 64 at a time.
@@ -446,7 +447,9 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const Args a) {
     g.mx = top;
     g.c = 1.0 / (LN2_32 * (double)temp);
     g.md = (double)g.mx;
-    g.bins = (float)fmin((double)NB / RANGE / (double)temp, 1e30);
+    // (differences of logits pass a float's range where they are as large as floats get; bins, where the temperature is as small)
+    g.by = temp < 0x1p-60f ? 0x1p60f : 0.5f;
+    g.bins = (float)((double)NB / RANGE / (double)temp / (double)g.by);
     g.tab = s.tab;
     g.keys = nullptr;
     const double least = fmin((double)(a.min_p ? a.min_p[r] : a.min_p_all), 1.0) * W1;
@@ -527,7 +530,7 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const Args a) {
     // (a little below what min-p leaves, in logits: the weight itself decides)
     float rough = zero;
     if (least > 0.0) {
-        const float f = (float)((double)top + (double)temp * (log(least / W1) - 1e-3)) - fabsf(top) * 0x1p-22f;
+        const float f = of_key(key_of((float)((double)top + (double)temp * (log(least / W1) - 1e-3)) - fabsf(top) * 0x1p-22f) - 1);     // (and the rounding)
         if (f > zero && f < top) rough = f;
     }
     auto weight = [&](float x) -> u64 {

@@ -48,3 +48,30 @@ def test_numbers_next_to_a_border(H, dt, V):
     check(H, x.cuda(), u, temp)
     # the order is (1, 0): token 0 is kept by top-p if w(1) <= p (w(0) + w(1))
     check(H, x.cuda(), torch.full_like(u, 0.01), temp, p=1 - u)
+
+
+@pytest.mark.parametrize("V", [40, 30000])
+@pytest.mark.parametrize("temp", [1e-45, 1e-38, 1e-30, 3e-20, 1e-10, 1e10, 1e30, 1e37, 3e38, math.inf])
+def test_temperatures_of_any_size(H, V, temp):
+    """Logits that differ by a few temperatures, however small or large those are: as far as floats go."""
+    g = torch.Generator().manual_seed(V)
+    t = torch.full((24,), temp)                                        # the float that the row gets
+    unit = float(t[0]) if math.isfinite(temp) else 1e38
+    x = -torch.rand(24, V, generator=g, dtype=torch.float64) * 40 * unit
+    x = torch.clamp(x, -3.4e38, 3.4e38).to(torch.float32)
+    x[:, V // 2] = 0.0
+    x[::3, 5::7] = -math.inf
+    if temp <= 1e-10:                                                  # the largest far from 0 would take the differences' bits
+        x[1::3] *= 0.5
+        if temp <= 1e-30:                                              # far more temperatures below the largest, all the same near it
+            x[2::3, ::2] = (-1e-27 * torch.rand(8, (V + 1) // 2, generator=g, dtype=torch.float64)).to(torch.float32)
+            x[2::3, V // 2] = 0.0
+    elif temp >= 1e37:                                                 # above and below 0: differences past the largest float
+        x[1::3] = ((torch.rand(8, V, generator=g, dtype=torch.float64) - 0.5) * 6.6e38).to(torch.float32)
+    u = torch.rand(24, generator=g)
+    check(H, x.cuda(), u, t)
+    check(H, x.cuda(), u, t, k=7)
+    check(H, x.cuda(), u, t, p=0.7)
+    for m in (0.05, 0.3, math.exp(-6.3)):
+        check(H, x.cuda(), u, t, m=m)
+    check(H, x.cuda(), u, t, k=V // 2, p=0.9, m=0.001)
