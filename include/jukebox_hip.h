@@ -297,7 +297,7 @@ int jb_sample_step(const float* logits, int n_batch, int bins, const jb_sample_p
  * the sum, min-p -- lies within that error of a weight or sum; weights below 2^-45 (logits 31.2 temp under the largest) are 0. */
 typedef struct jb_sample_filtered_args {
     int dtype;                                         /* JB_F32, JB_F16, JB_BF16 */
-    const void* logits; int64_t ld; int rows, bins;    /* [rows] of ld elements, bins of them logits */
+    const void* logits; int64_t ld; int rows, bins;    /* [rows] of ld elements, bins of them logits; ld 0: every row the same one */
     const float* u;                                    /* [rows], in [0, 1) */
     const float* temp; const int* top_k; const float *top_p, *min_p;              /* [rows] each, or NULL: */
     float temp_all; int top_k_all; float top_p_all, min_p_all;                    /* the value of every row */

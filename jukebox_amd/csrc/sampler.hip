@@ -619,20 +619,27 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const Args a) {
 extern "C" int jb_sample_filtered(const jb_sample_filtered_args* a, void* stream) {
     JB_REQUIRE(a, "null pointer");
     JB_REQUIRE(a->dtype == JB_F32 || a->dtype == JB_F16 || a->dtype == JB_BF16, "bad dtype");
-    JB_REQUIRE(a->rows >= 0 && a->bins > 0 && (a->ld >= a->bins || a->rows < 2), "bad dims");
+    JB_REQUIRE(a->rows >= 0 && a->bins > 0 && (a->ld >= a->bins || a->ld == 0 || a->rows < 2), "bad dims");
     if (a->bins > MAX_BINS) JB_UNSUPPORTED("vocabularies of up to 262144 tokens");
     if (a->rows == 0) return JB_OK;
     JB_REQUIRE(a->logits && a->u && a->tokens, "null pointer");
-    const Args k = {a->logits, a->ld, a->bins, a->u, a->temp, a->top_k, a->top_p, a->min_p, a->temp_all, a->top_k_all, a->top_p_all, a->min_p_all, a->tokens};
     hipStream_t s = (hipStream_t)stream;
-    // rows of up to 16384 tokens: four waves, whose barriers cost less than the other twelve would save
-#define JB_GO(T)                                                                                   \
-    do {                                                                                           \
-        if (a->bins <= 16384) sample_filtered_kernel<T, 256><<<(unsigned)a->rows, 256, 0, s>>>(k); \
-        else sample_filtered_kernel<T, 1024><<<(unsigned)a->rows, 1024, 0, s>>>(k);                \
+    constexpr int64_t MOST = 1 << 21;                  // rows of a launch, which holds 2^32 threads
+    for (int64_t r = 0; r < a->rows; r += MOST) {
+        const unsigned n = (unsigned)(a->rows - r < MOST ? a->rows - r : MOST);
+        const char* row = (const char*)a->logits + r * a->ld * (a->dtype == JB_F32 ? 4 : 2);
+        auto from = [&](auto* p) { return p ? p + r : p; };
+        const Args k = {row, a->ld, a->bins, a->u + r, from(a->temp), from(a->top_k), from(a->top_p), from(a->min_p),
+                        a->temp_all, a->top_k_all, a->top_p_all, a->min_p_all, a->tokens + r};
+        // rows of up to 16384 tokens: four waves, whose barriers cost less than the other twelve would save
+#define JB_GO(T)                                                                  \
+    do {                                                                          \
+        if (a->bins <= 16384) sample_filtered_kernel<T, 256><<<n, 256, 0, s>>>(k); \
+        else sample_filtered_kernel<T, 1024><<<n, 1024, 0, s>>>(k);               \
     } while (0)
-    if (a->dtype == JB_F32) JB_GO(float); else if (a->dtype == JB_F16) JB_GO(f16); else JB_GO(bf16);
+        if (a->dtype == JB_F32) JB_GO(float); else if (a->dtype == JB_F16) JB_GO(f16); else JB_GO(bf16);
 #undef JB_GO
-    JB_CHECK_LAUNCH();
+        JB_CHECK_LAUNCH();
+    }
     return JB_OK;
 }

@@ -560,7 +560,7 @@ def make_sample_params(temp=1.0, top_k=0, top_p=0.0, seed=0, sample_base=0, pos_
 def sample_filtered(logits, u, temp=1.0, top_k=0, top_p=0.0, min_p=0.0, out=None):
     """One token a row (int64) from given uniform numbers after temperature, top-k, top-p and min-p (jb_sample_filtered has the
     definition, which the answer equals whatever the sizes).  logits (rows, bins), float32, float16 or bfloat16, rows of any
-    pitch; u (rows) float32 in [0, 1).  temp, top_k, top_p, min_p: a number for all rows or an array with one for each (int32 for
+    pitch that does not overlap them, or one row expanded to many; u (rows) float32 in [0, 1).  temp, top_k, top_p, min_p: a number for all rows or an array with one for each (int32 for
     top_k, float32 for the others).  temp <= 0: the largest logit; top_k <= 0, top_p <= 0 or >= 1, min_p <= 0: off.  -inf and NaN
     are forbidden tokens; a row without any other gives -1."""
     code = _paged_type(logits)

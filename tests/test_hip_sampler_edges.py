@@ -75,3 +75,38 @@ def test_temperatures_of_any_size(H, V, temp):
     for m in (0.05, 0.3, math.exp(-6.3)):
         check(H, x.cuda(), u, t, m=m)
     check(H, x.cuda(), u, t, k=V // 2, p=0.9, m=0.001)
+
+
+def test_more_rows_than_a_launch_holds(H):
+    n = (1 << 24) + 5
+    g = torch.Generator("cuda").manual_seed(3)
+    x = torch.randn(n, 2, generator=g, device="cuda").half()
+    got = H.sample_filtered(x, torch.zeros(n, device="cuda"), 0.0)
+    assert torch.equal(got, (x[:, 1] > x[:, 0]).long())
+
+
+@pytest.mark.parametrize("dt,V,n", [("f32", 300, 5000), ("bf16", 17000, (1 << 22) + 3), ("f16", 2048, 1)])
+def test_one_row_drawn_from_many_times(H, dt, V, n):
+    """A row expanded to n of them (a pitch of 0), each with a number and a temperature of its own."""
+    g = torch.Generator("cuda").manual_seed(V)
+    # two temperatures: at 0.5 the weights of these logits are squares of those at 1
+    row = torch.randint(0, 12, (1, V), generator=g, device="cuda").double()
+    x = (row * math.log(2.0)).to(TYPES[dt])
+    u = torch.rand(n, generator=g, device="cuda")
+    temp = torch.where(torch.rand(n, generator=g, device="cuda") < 0.5, 0.5, 1.0)
+    got = H.sample_filtered(x.expand(n, V), u, temp)
+    for t in (0.5, 1.0):
+        rows = temp == t
+        if not bool(rows.any()):
+            continue
+        w = torch.exp((x[0].double() - x.double().max()) / t)
+        cum = torch.cumsum(w, 0)
+        goal = u[rows].double() * cum[-1]
+        # (rows whose number falls onto a border, to the two sums' own rounding, are left out)
+        i = torch.searchsorted(cum, goal, right=True)
+        near = torch.minimum((cum[i] - goal).abs(), (goal - torch.where(i > 0, cum[(i - 1).clamp(min=0)], goal - 1)).abs()) < 1e-9 * cum[-1]
+        assert bool(((got[rows] == i) | near).all()) and float(near.double().mean()) < 1e-3
+    if n > 1000:
+        full = x.expand(1000, V).contiguous()
+        assert torch.equal(got[:1000], H.sample_filtered(full, u[:1000].contiguous(), temp[:1000].contiguous()))
+        assert torch.equal(got[-1000:], H.sample_filtered(full, u[-1000:].contiguous(), temp[-1000:].contiguous()))
