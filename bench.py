@@ -8,7 +8,7 @@ seeded random-init weights of the released architecture (no checkpoints are reac
 
 A "step" is one full pass of the hot path over one batch: all three levels for 16 samples per GPU (n_samples is sharded
 over the ranks, weak scaling) -- minutes of GPU time.  The run therefore works against a WALL BUDGET (JB_BENCH_BUDGET_S,
-default 1400 s from process start, model build included): at most one short untimed warm-up pass, then full-length timed
+default 540 s from process start, model build included): at most one short untimed warm-up pass, then full-length timed
 steps while another one still fits, at least one and at most --steps.  The JSON line reports the steps actually timed
 (`steps`, `ms_per_step`) next to the requested counts, so a driver command such as `--steps 20 --warmup 5` always
 yields a line.  Rank 0 prints ONE JSON line.
@@ -77,7 +77,7 @@ from jukebox_amd.utils import dist_adapter as dist  # noqa: E402
 from jukebox_amd.utils.dist_utils import setup_dist_from_env, shard_range  # noqa: E402
 
 _JSON_OUT = sys.stdout
-BUDGET_S = float(os.environ.get("JB_BENCH_BUDGET_S", "1400"))
+BUDGET_S = float(os.environ.get("JB_BENCH_BUDGET_S", "540"))
 T_ORIGIN = float(os.environ.get("JB_BENCH_T0", repr(T_PROC)))
 
 

@@ -287,7 +287,9 @@ int jb_sample_step(const float* logits, int n_batch, int bins, const jb_sample_p
 
 /* One token a row from given uniform numbers: temperature, then top-k, top-p and min-p, then the draw -- what jb_sample_logits does
  * with a generator of its own, one filter at a time and up to 4096 bins (filter_logits, jukebox/transformer/ops.py:113-142), for any
- * vocabulary of up to 262144 tokens, every row with settings of its own.  With w_i = exp((x_i - max) / temp) and the row ordered by
+ * vocabulary of up to 262144 tokens, every row with settings of its own.  (Among equal logits at the last kept place jb_sample_logits
+ * keeps all, as the filter by a threshold does; this keeps the lowest indices, k of them in top-k, which in 16 bits, where logits are often
+ * equal, is another set.)  With w_i = exp((x_i - max) / temp) and the row ordered by
  * falling logit, equal ones by rising index: top-k keeps the first k (k <= 0 or >= bins: off); top-p, of those, each entry before
  * which the weights sum to at most p of theirs (p <= 0 or >= 1: off); min-p those with w_i >= min_p (<= 0: off; above 1 is 1).
  * The token is the first index at which the sum of kept weights, by rising index, exceeds u times their total.  temp <= 0: the

@@ -110,3 +110,14 @@ def test_one_row_drawn_from_many_times(H, dt, V, n):
         full = x.expand(1000, V).contiguous()
         assert torch.equal(got[:1000], H.sample_filtered(full, u[:1000].contiguous(), temp[:1000].contiguous()))
         assert torch.equal(got[-1000:], H.sample_filtered(full, u[-1000:].contiguous(), temp[-1000:].contiguous()))
+
+
+def test_equal_logits_at_the_border_of_two_samplers(H):
+    """Four equal logits and top-k 2: jb_sample_logits draws from all four, as a threshold keeps them; this from the two lowest indices."""
+    n = 256
+    x = torch.full((n, 64), -3.0, device="cuda")
+    x[:, [7, 20, 33, 50]] = 1.0
+    tokens, t_dev = torch.zeros(n, 1, dtype=torch.int64, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    H.sample_logits(x, H.make_sample_params(top_k=2, seed=5), tokens, t_dev)
+    assert set(tokens[:, 0].tolist()) == {7, 20, 33, 50}
+    assert set(H.sample_filtered(x, torch.rand(n, device="cuda"), top_k=2).tolist()) == {7, 20}
