@@ -15,7 +15,7 @@ SOURCES = ["api.hip", "gemm.hip", "attention.hip", "elementwise.hip", "engine.hi
 # forms have given wrong results on this hardware now and then, without an error
 FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # the attention over pages keeps its accumulators in the vector registers proper (the compiler else moves every matrix instruction's
-# result of a kernel of more than 256 registers through the accumulation registers: chunks of 256-channel heads 269 -> 226 us)
+# result of a kernel of more than 256 registers through the accumulation registers: chunks of 256-channel heads 305 -> 248 us)
 SOURCE_FLAGS = {"paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 HEADERS = ["common.h", "paged.h", "gemm_glds_index.h", "gemm_8phase.h", os.path.join("..", "..", "include", "jukebox_hip.h")]
 LIB = os.path.join(HERE, "libjukebox_hip.so")

@@ -253,10 +253,10 @@ __device__ void put_infinities(const Args& a, const Seq& s, const Tile& t, int k
 // ALIGNED (pages of a multiple of 16 rows, keys at consecutive positions): a 16-key half of a turn lies in one page, so that its rows
 // are one scalar address and a lane's constant offset, page numbers come 64 at a time, and the next turn's rows are on their way while
 // one is computed.  Otherwise (odd pages, the transpose pattern) every key is looked up by a lane and its address handed round.
-// Measured (one new token a sequence; a copy reaches 4.8 TB/s on the card): 64 sequences of 511-8192 keys, 32 heads on 8 of 128 channels,
-// bf16 in pages of 16: 261 us, 4.4 TB/s; 16 of 4096-8192 under a head of 480, f16: 43 us, 4.4 TB/s; 64 of 500-4000, 8 heads of 150: 171 us, 4.1 TB/s.
-// Bound by memory.  Three waves a SIMD instead of two, for which the registers spill: 353, 61 and 259 us.  Keys looked up lane by lane
-// instead of ALIGNED: 345, 70 and 350 us.
+// Measured (one new token a sequence; a copy reaches 4.7 TB/s on the card): 64 sequences of 511-8192 keys, 32 heads on 8 of 128 channels,
+// bf16 in pages of 16: 260 us, 4.4 TB/s; 16 of 4096-8192 under a head of 480: 39 us in f16, 4.8 TB/s over and over the same cache (4.0 over
+// three in turn), 94 us in f32, 4.0 TB/s; 64 of 500-4000, 8 heads of 150: 178 us, 3.8 TB/s.  Bound by memory.  Three waves a SIMD instead of
+// two, for which the registers spill: 310, 54, 174 and 289 us.  Keys looked up lane by lane instead of ALIGNED: 251, 43, 125 and 263 us.
 template <typename T, int NC> struct Shape {
     static constexpr int WAVES = NC > 4 ? NC : 4, KG = WAVES / NC, CH = 16 * El<T>::E, LDO = CH + 4;     // LDO: rows 4 banks apart
     struct alignas(16) Shared {
@@ -631,12 +631,13 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
 // permutations ([channel][key], so that an operand is one 16-byte read), all asked for a turn ahead.  LDS rows are padded by 16 bytes: the
 // 16 lanes of a read phase then hit 16 different groups of four banks.
 // The probabilities enter the second product rounded once to 16 bits, which adds an error of the size of the output's own
-// rounding (each is off by half a step, and they average); a second product for the rest would cost a quarter of the rate.
+// rounding (each is off by half a step, and they average); a second product for the rest took 864 us for 707 of the second case below.
 // Measured (32 heads on 8 of 128 channels, bf16, pages of 64; the library's product of 16384^3 runs at 1370 TFLOP/s): 4 x 2048 queries behind
-// 6144 keys: 1.22 ms, 790 TFLOP/s; 4 x 257-2048 behind 4097-8192: 670-750 us from card to card, 630-700
-// TFLOP/s; 8 heads of 150, f16, 100-1000 queries behind 1000-5000: 120 us, 244 TFLOP/s.  Two workgroups share a compute unit, and the
-// products' 27 % of the time hide behind the softmax's exponentials and the LDS reads, of which either alone would take about as long
-// as the products at their peak.  Waves of 64 rows, which halve the LDS reads but leave one wave a SIMD (and its registers spilling): 1.13 ms
+// 6144 keys: 1.20-1.26 ms, 760-800 TFLOP/s; 4 x 257-2048 behind 4097-8192: 690-760 us from card to card, 620-690 TFLOP/s; 8 heads of 150, f16,
+// 100-1000 queries behind 1000-5000: 118 us, 247 TFLOP/s; 2 heads of 256, f16, 4 x 512-2048 behind 4096-6144: 250 us, 200 TFLOP/s.  Two workgroups
+// share a compute unit (one under 256 channels).  By the counters of the second case the matrix units are busy 27 % of the time, the vector
+// ALU issues -- the softmax's exponentials, most of all -- 39 %, the LDS is read 24 %: two waves a SIMD overlap little of them, and the
+// registers hold no third.  Waves of 64 rows, which halve the LDS reads but leave one wave a SIMD (and its registers spilling): 1.13 ms
 // instead of 0.83 for the second case as things then were.
 template <typename T> struct Mfma32;
 template <> struct Mfma32<f16> { static __device__ __forceinline__ f32x16 go(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); } };
@@ -1000,16 +1001,16 @@ Plan plan_of(const jb_attn_paged_args* p) {
     w.splits = 1; w.chunk = 0x7fffffff;
     int64_t chunk = 0;
     // Few tiles: the keys are split, so that every compute unit has two workgroups.  A workgroup costs some 5 us before its first keys
-    // are there, so its turn is 256 keys at least (16 sequences of 4096-8192 keys under one head of 480: 43 us; 512 keys: 55, 128: 58) -- a
-    // launch too small to fill the chip even so takes 64 (300 keys: 17 us against 32) -- and 2048 at most, which evens out
-    // sequences of different lengths (64 of 511-8192 keys: 261 us against 267 unsplit).
+    // are there, so its turn is 256 keys at least (16 sequences of 4096-8192 keys under one head of 480: 39 us; 512 keys: 43, 128: 45) -- a
+    // launch too small to fill the chip even so takes 64 (300 keys: 17 us against 27) -- and 2048 at most, which evens out
+    // sequences of different lengths (64 of 511-8192 keys: 260 us against 266 unsplit).
     if (w.tr == 16 && wgs < 1024 && w.range > 64) {
         chunk = (wgs * w.range / 512 + 127) / 128 * 128;
         if (chunk > 2048) chunk = 2048;
         if (chunk < 256) chunk = wgs * w.range <= 64 * 256 ? 64 : 256;
     }
     // Chunks: two workgroups a compute unit as well, by the tiles that there can be in all (sequences are rarely as long as the longest:
-    // 3 of 100-1000 queries, 5000 keys under 8 heads of 150: 120 us, split for as many tiles as the launch has 168; 1000 queries of one
+    // 3 of 100-1000 queries, 5000 keys under 8 heads of 150: 118 us, split for as many tiles as the launch has 168; 1000 queries of one
     // sequence: 80 us; three or four workgroups a unit: 103; one and a half: 95), and 512 keys at least.
     const int64_t filled = (p->n_tokens * G + w.tr - 1) / w.tr + p->n_seq / 2, real = filled * p->n_kv_head < wgs ? filled * p->n_kv_head : wgs;
     if (w.tr > 16 && real < 1024 && w.range > 512) {
