@@ -395,7 +395,7 @@ __global__ __launch_bounds__((Shape<T, NC>::WAVES * 64), 2) void attn_paged_rows
                         // the top bit of an element: all of its exponent's are set (an addition carries into it)
                         const unsigned bad = ((w & El<T>::ABS) + El<T>::STEP) & ~El<T>::ABS;
                         vf[i][h] = w & ~(E == 8 ? (bad - (bad >> 15)) | bad : (unsigned)((int)bad >> 31));
-                        odd |= bad != 0u;
+                        odd |= bad != 0u && nk > 0;                            // (a slice behind the head's end has loaded none)
                     }
                 }
             }
