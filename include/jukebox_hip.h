@@ -328,7 +328,9 @@ int jb_vq_argmin(const float* x, const float* xk, const float* codebook, int64_t
  * fixed length per sample (FactoredAttention.forward(sample=True), jukebox/transformer/factored_attention.py:82-193,289-301).
  * Rows cu_q[i] .. cu_q[i+1]-1 of q [n_tokens][n_head][d_head] are sequence i's; rows outside every sequence are neither read
  * nor written; out overlaps no input.  n_head / n_kv_head consecutive query heads share a key / value head.  A query without a visible key (block 0
- * of the prev pattern, a length below the number of queries) gives zeros; a masked key or value may hold anything, NaN too;
+ * of the prev pattern, a length below the number of queries, scores of -inf alone) gives zeros; a masked key or value may hold anything,
+ * NaN too; an infinite value that a query sees makes its output infinite, ones of both signs or a NaN make it no number, also where that
+ * key's score is -inf;
  * positions whose table entry is no page number are masked.  Patterns 0-3; `window` (dense only, 0 = off): the query at p sees
  * positions p - window + 1 .. p.  Strides in elements, channels contiguous; k and v share them.  Scores, softmax and sums in fp32;
  * 16-bit outputs are rounded once.  In 16 bits a probability enters the value product as the sum of two numbers of the type (off by

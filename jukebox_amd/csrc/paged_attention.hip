@@ -184,7 +184,8 @@ template <typename T> __device__ __forceinline__ void store8(T* o, const float* 
 }
 
 // Values that are no numbers, for the 16 rows of a tile from row0 on that are not in `skip`: where a row sees an infinite value its output is
-// infinite, where it sees infinite ones of both signs or a NaN it is no number, whatever else is in the sum (a probability is never 0).  The
+// infinite, where it sees infinite ones of both signs or a NaN it is no number, whatever else is in the sum (a probability is not 0; one of a
+// score of -inf is, and 0 times infinity no number: its key counts all the same, as telling it took 5-10 % of short chunks' time).  The
 // matrix products cannot say so: a value a row does not see would reach it as 0 * NaN, and one that it sees meets parts that are 0 -- the low
 // part of a probability that has none, a probability that rounds to 0.  So turns that some row does not see whole take such values out of
 // the operands, and a tile that has met one, or whose sums are not finite, ends here: one wave looks through the split's values, 64
