@@ -344,3 +344,21 @@ def test_a_step_without_max_q(H):
         assert torch.equal(b.run(H), b.run(H, max_q=1))
         want, tol = Made.fine(b)
         assert bool(((b.run(H).double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dt", sorted(TYPES))
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-3, 2.0])
+@pytest.mark.parametrize("heads,kv,D", [(2, 2, 9), (2, 1, 12), (1, 1, 15), (2, 2, 23), (2, 2, 150), (1, 1, 200), (1, 1, 255), (1, 1, 301)])
+def test_scales_and_odd_widths(H, dt, scale, heads, kv, D):
+    """Negative, zero and large scales; heads whose last piece repeats 1 to 7 channels, in one piece more than they fill and in many."""
+    for lens, nq, page in (([90, 33], [1, 1], 16), ([300, 20], [80, 20], 7), ([700], [100], 64)):
+        Batch(TYPES[dt], lens, nq, heads, kv, D, page, seed=D).check(H, scale=scale)
+
+
+def test_a_table_that_is_part_of_a_wider_one(H):
+    b = Batch(torch.bfloat16, [300, 41, 7], [70, 1, 3], 4, 2, 64, 16, seed=50)
+    wide = torch.full((3, b.table.shape[1] + 9), 10 ** 6, dtype=torch.int32, device="cuda")
+    wide[:, 4:4 + b.table.shape[1]] = b.table
+    want = b.run(H)
+    b.table = wide[:, 4:4 + b.table.shape[1]]
+    assert torch.equal(b.run(H), want)
