@@ -15,7 +15,8 @@
 // weights; the bin in which k or p is crossed, and among its few entries the last kept one; the kept weights by tiles of consecutive
 // indices; the tile that u falls into.  A row of 128000 16-bit logits is 256 KB, which its die's L2 keeps for the passes after the
 // first: memory's part of 256 such rows (65 MB) is 14 us.  Measured (256 x 128000 bf16, normal logits of deviation 2.5): no filter 40 us,
-// top-k 50 56, top-p 0.9 85, both 85, min-p 0.05 34; temperature 0 20; two thirds of the entries equal, top-p 131.  What bounds it is the exponential in double precision of every
+// top-k 50 56, top-p 0.9 85, both 85, min-p 0.05 34; temperature 0 20; two thirds of the entries equal, top-p 131, and temperature 0
+// 257 if they are the largest (their indices meet at one address).  What bounds it is the exponential in double precision of every
 // entry that is weighed (for 16-bit logits taken from a table in LDS instead: 120 -> 98 us with top-p when it came in) and the LDS atomics of the histogram.
 #include "paged.h"
 
